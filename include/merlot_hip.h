@@ -545,6 +545,51 @@ int64_t merlot_crc32c(uint64_t crc, const void* data, int64_t n, int force_sw);
 int64_t merlot_example_index(const void* buf, int64_t n, int64_t* rows, int64_t max_rows, int64_t* ivals, int64_t max_ivals,
                              float* fvals, int64_t max_fvals);
 
+/* ------------------------------------------------------------------------------------------------
+ * Root-mean-square norm, 8-bit blocks and their product, gradient clipping.  No counterpart in the reference (its norms are LayerNorm, its compute is bf16);
+ * added entries, so the ABI version stands.
+ * ---------------------------------------------------------------------------------------------- */
+/* h = round(x + residual), R = 1 / sqrt(mean(h^2) + eps), y = h * R * gamma over rows of H features, any H from 1 to 16 384; statistics fp32, taken from h
+ * AS STORED.  x, residual, h, y all bf16 (x_f32 0) or all f32; x and residual with row strides ldx / ldr >= H, h and y dense.  residual and h: both or neither
+ * (without them h is x).  y may be NULL when y8 is given; rstd (f32 [rows], = R) may be NULL when no backward follows.
+ * y8 / scale8 (optional): the e4m3 copy of the UNROUNDED y in blocks of 128 features, as merlot_quantize_blocks lays it out (ld8 = ceil(H / 128) * 128). */
+int merlot_rms_fwd(const void* x, int64_t ldx, int x_f32, const void* residual, int64_t ldr, const float* gamma, void* h, void* y, float* rstd,
+                   void* y8, int64_t ld8, uint8_t* scale8, int64_t ld_scale8, int64_t rows, int H, float eps, merlot_stream_t stream);
+/* dx = R * (dy * gamma - n * mean(dy * gamma * n)) (+ dres), n = h * R; dgamma[H] (f32) += sum over rows of dy * n, in a fixed order (no atomics).  dy, h, dres
+ * (may be NULL) and dx share one type; dx dense.  dx is the gradient of x and of the residual alike.  workspace: merlot_rms_bwd_workspace_bytes(rows, H), any content. */
+int64_t merlot_rms_bwd_workspace_bytes(int64_t rows, int H);
+int merlot_rms_bwd(const void* dy, int64_t lddy, int is_f32, const void* h, int64_t ldh, const float* rstd, const float* gamma, const void* dres,
+                   int64_t lddr, void* dx, float* dgamma, int64_t rows, int H, void* workspace, int64_t workspace_bytes, merlot_stream_t stream);
+
+/* 8-bit copies of x [R, C] (bf16 or f32, row stride ldx) in blocks of 128, one or both of
+ *   q  [R, ldq]  codes, blocks along the columns, columns C .. ceil(C / 128) * 128 zero;   s  [R, lds]:  scale byte of block b of row r at r * lds + b
+ *   qt [C, ldqt] the transposed codes, blocks along the ROWS of x, padded likewise;         st [C, ldst]
+ * fmt 0 = e4m3, 1 = e5m2.  A scale byte b stands for 2^(b - 127): the least power of two (not under 2^-127) that brings the block's max |x| to at most the
+ * format's largest value; 2^0 for a block of zeros.  A block that holds an infinity or NaN becomes NaN as a whole (byte 255, codes NaN).  Dividing by a power of
+ * two is exact, so a copy's value is x rounded once, and never saturates.
+ * tile 1: a scale per row (of q, of qt) and block; tile 128: one scale per 128 x 128 tile, repeated for its rows -- q and qt then hold the same values. */
+int merlot_quantize_blocks(const void* x, int64_t ldx, int x_f32, int64_t R, int64_t C, int fmt, int tile, void* q, int64_t ldq, uint8_t* s,
+                           int64_t lds, void* qt, int64_t ldqt, uint8_t* st, int64_t ldst, merlot_stream_t stream);
+/* C[M,N] (+)= sum over blocks b of 128 of 2^(scale_a[m,b] - 127 + scale_b[n,b] - 127) * (A8[m,b] . B8[n,b]) (+ bias[n]): operands as merlot_quantize_blocks
+ * writes them, A8 e4m3 (fmt_a 0) or e5m2 (1), B8 e4m3; K % 128 == 0, M and N any; operand rows 16-byte, scale rows 4-byte aligned (leading dimensions too) and
+ * read in whole words of 4 bytes.  fp32 accumulators; an f32 C is good to fp32 (the codes go through the bf16 matrix instruction, exactly), a bf16 C comes from the
+ * 8-bit instruction, which keeps 13 bits below the largest of each eight products.  C bf16 or f32 (out_f32; accumulate adds into C before the one rounding), ldc any.  bias f32 [N] or NULL.
+ * workspace: merlot_gemm_f8_blocks_workspace_bytes(M, N, K) bytes, 16-byte aligned, any content (partial products of reductions that are split over workgroups and
+ * folded in a fixed order; may be NULL where that is 0). */
+int64_t merlot_gemm_f8_blocks_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int merlot_gemm_f8_blocks(const void* A8, int64_t lda, int fmt_a, const uint8_t* scale_a, int64_t ld_scale_a, const void* B8, int64_t ldb,
+                          const uint8_t* scale_b, int64_t ld_scale_b, void* C, int64_t ldc, int64_t M, int64_t N, int64_t K, int out_f32,
+                          int accumulate, const float* bias, void* workspace, int64_t workspace_bytes, merlot_stream_t stream);
+
+/* norm[0] (f32) = sqrt(sum over n tensors of sum of g^2), summed in 64 bits in a fixed order, and with clip > 0 out = g * (clip / max(norm, clip)) -- the
+ * arithmetic of tf.clip_by_global_norm (utils/optimization.py:233-237); clip 0: the norm alone, `out` may be NULL.  in / out / numel / types: HOST arrays of n
+ * device addresses, element counts (0 allowed) and types (bit 0: in is bf16, bit 1: out is bf16; otherwise f32); addresses aligned to their type.  out[i] == in[i]
+ * of the same type works in place; outputs that overlap each other or another tensor's input are refused.  A norm that is not finite is passed on: infinity
+ * scales by 0, NaN by NaN.  workspace: merlot_clip_workspace_bytes(n) bytes, 8-byte aligned, any content. */
+int64_t merlot_clip_workspace_bytes(int64_t n);
+int merlot_clip_by_global_norm(const int64_t* in, const int64_t* out, const int64_t* numel, const uint8_t* types, int64_t n, float clip, float* norm,
+                               void* workspace, int64_t workspace_bytes, merlot_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -8,8 +8,8 @@ cd "$(dirname "$0")"
 HIPCC=${HIPCC:-/opt/rocm/bin/hipcc}
 # packed fp32 instructions stay off: some forms of v_pk_{add,mul,fma}_f32 have given wrong results on this hardware now and then
 FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Xclang -target-feature -Xclang -packed-fp32-ops -Wall -Wno-unused-function -Wno-unused-variable"
-SRCS="gemm attention layernorm elementwise index conv conv_gemm image fp8 jpeg"
-HDRS="common.h gemm_ring.h gemm_p8.inc gemm_q8.inc attention_res.inc attention_fb.inc attention_pp.inc ../../include/merlot_hip.h"
+SRCS="gemm attention layernorm elementwise index conv conv_gemm image fp8 jpeg rmsnorm blocks8 gemm_blocks clip"
+HDRS="common.h blocks8.h gemm_ring.h gemm_p8.inc gemm_q8.inc attention_res.inc attention_fb.inc attention_pp.inc ../../include/merlot_hip.h"
 
 newer() {  # newer <target> <deps...>: true when target is missing or older than a dependency
   local t=$1; shift

@@ -1,0 +1,300 @@
+// Root-mean-square norm for gfx950, forward (with the residual's addition and an 8-bit copy of the output) and backward.
+//
+//   h = round(x + residual);  R = 1 / sqrt(mean(h^2) + eps);  y = h * R * gamma
+//   n = h * R;  t = dy * gamma;  dx = R * (t - n * mean(t * n)) (+ dres);  dgamma += sum over rows of dy * n
+//
+// Both directions are bound by memory: every operand crosses it once.  A row is held in registers by WPR waves (1 up to 2 048 features, 4 above), each lane
+// VEC consecutive features per slab, so a lane's loads and stores are 8 or 16 bytes and the 128 features that share a scale lie in 128 / VEC neighbouring lanes.
+// All sums are fp32.  The statistics are taken from h AS STORED (rounded to its type), so that the backward, which reads the stored h, differentiates the
+// function the forward computed.
+#include "common.h"
+#include "blocks8.h"
+
+namespace {
+
+// VEC consecutive elements at any element alignment (gfx950 loads and stores global dwords at byte alignment): rows of odd width need no path of their own
+template <typename T, int VEC> struct ElemVec { typedef T type __attribute__((ext_vector_type(VEC), aligned(sizeof(T)))); };
+
+// `left`: how many of the VEC elements exist (may be <= 0)
+template <typename T, int VEC>
+__device__ __forceinline__ void load_vec(const T* p, int left, float (&v)[VEC]) {
+    if (left >= VEC) {
+        const typename ElemVec<T, VEC>::type t = *reinterpret_cast<const typename ElemVec<T, VEC>::type*>(p);
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = (float)t[e];
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = e < left ? (float)p[e] : 0.f;
+    }
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_vec(T* p, int left, const float (&v)[VEC]) {
+    if (left >= VEC) {
+        typename ElemVec<T, VEC>::type t;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) t[e] = (T)v[e];
+        *reinterpret_cast<typename ElemVec<T, VEC>::type*>(p) = t;
+    } else {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e)
+            if (e < left) p[e] = (T)v[e];
+    }
+}
+
+// sum over the row's WPR waves.  slot: which of the alternating LDS rows this call uses -- a wave may be one call ahead of another, never two.
+template <int WPR>
+__device__ __forceinline__ float row_sum(float s, float (*red)[WPR], int& slot) {
+    s = wave_sum(s);
+    if constexpr (WPR > 1) {
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) red[slot][wave] = s;
+        __syncthreads();
+        s = 0.f;
+#pragma unroll
+        for (int w = 0; w < WPR; ++w) s += red[slot][w];
+        slot ^= 1;
+    }
+    return s;
+}
+
+struct RmsFwdArgs {
+    const void* x; int64_t ldx;
+    const void* res; int64_t ldr;
+    const float* gamma;
+    void *h, *y;                 // dense [rows, H]; h only with res
+    float* rstd;
+    uint8_t* y8; int64_t ld8;    // dense columns up to whole blocks of 128
+    uint8_t* s8; int64_t lds8;
+    int64_t rows; int H; float eps;
+};
+
+template <typename T, int VEC, int NS, int WPR, bool RES>
+__global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwdArgs p) {
+    constexpr int RPB = 4 / WPR;                         // rows in flight per workgroup
+    __shared__ float red[2][WPR];
+    int slot = 0;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c0 = ((wave % WPR) * 64 + lane) * VEC;     // this lane's first feature of a slab
+    constexpr int SLAB = WPR * 64 * VEC;
+    const int H = p.H;
+    const T* x = (const T*)p.x;
+    const T* res = (const T*)p.res;
+    for (int64_t row = (int64_t)blockIdx.x * RPB + wave / WPR; row < p.rows; row += (int64_t)gridDim.x * RPB) {
+        float v[NS][VEC];
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int c = i * SLAB + c0;
+            load_vec<T, VEC>(x + row * p.ldx + c, H - c, v[i]);
+            if constexpr (RES) {
+                float r[VEC];
+                load_vec<T, VEC>(res + row * p.ldr + c, H - c, r);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) v[i][e] = (float)(T)(v[i][e] + r[e]);
+                store_vec<T, VEC>((T*)p.h + row * H + c, H - c, v[i]);
+            }
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) ss += v[i][e] * v[i][e];
+        }
+        ss = row_sum<WPR>(ss, red, slot);
+        const float rstd = 1.0f / sqrtf(ss / (float)H + p.eps);
+        if (p.rstd && lane == 0 && wave % WPR == 0) p.rstd[row] = rstd;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int c = i * SLAB + c0;
+            float g[VEC];
+            load_vec<float, VEC>(p.gamma + c, H - c, g);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[i][e] = v[i][e] * rstd * g[e];
+            if (p.y) store_vec<T, VEC>((T*)p.y + row * H + c, H - c, v[i]);
+            if (p.y8) {                                  // from the unrounded y: ONE rounding between it and the 8-bit value
+                uint32_t m = 0;
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) m = max(m, __float_as_uint(v[i][e]) & 0x7fffffffu);
+                m = group_umax<128 / VEC>(m);
+                const int byte = block_scale_byte(m, E4M3_TOP);
+                if (c < p.ld8) {
+                    store_codes<0, VEC>(p.y8 + row * p.ld8 + c, v[i], byte);
+                    if ((c & 127) == 0) p.s8[row * p.lds8 + (c >> 7)] = (uint8_t)byte;
+                }
+            }
+        }
+    }
+}
+
+struct RmsBwdArgs {
+    const void* dy; int64_t lddy;
+    const void* h; int64_t ldh;
+    const float *rstd, *gamma;
+    const void* dres; int64_t lddr;
+    void* dx;                    // dense [rows, H]
+    float* part;                 // [gridDim.x, H]: each workgroup's sums of dy * n
+    int64_t rows; int H;
+};
+
+template <typename T, int VEC, int NS, int WPR>
+__global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdArgs p) {
+    constexpr int RPB = 4 / WPR;
+    constexpr int SLAB = WPR * 64 * VEC;
+    __shared__ float red[2][WPR];
+    __shared__ float gred[RPB > 1 ? RPB : 1][RPB > 1 ? SLAB : 1];
+    int slot = 0;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int c0 = ((wave % WPR) * 64 + lane) * VEC;
+    const int H = p.H;
+    const T* dy = (const T*)p.dy;
+    const T* h = (const T*)p.h;
+    const T* dres = (const T*)p.dres;
+    float dg[NS][VEC];
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) dg[i][e] = 0.f;
+    for (int64_t row = (int64_t)blockIdx.x * RPB + wave / WPR; row < p.rows; row += (int64_t)gridDim.x * RPB) {
+        const float rs = p.rstd[row];
+        float n[NS][VEC], t[NS][VEC];
+        float c1 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int c = i * SLAB + c0;
+            float g[VEC];
+            load_vec<T, VEC>(h + row * p.ldh + c, H - c, n[i]);
+            load_vec<T, VEC>(dy + row * p.lddy + c, H - c, t[i]);
+            load_vec<float, VEC>(p.gamma + c, H - c, g);
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                n[i][e] *= rs;
+                dg[i][e] += t[i][e] * n[i][e];
+                t[i][e] *= g[e];
+                c1 += t[i][e] * n[i][e];
+            }
+        }
+        c1 = row_sum<WPR>(c1, red, slot) / (float)H;
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const int c = i * SLAB + c0;
+            float o[VEC];
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) o[e] = rs * (t[i][e] - n[i][e] * c1);
+            if (dres) {
+                float r[VEC];
+                load_vec<T, VEC>(dres + row * p.lddr + c, H - c, r);
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) o[e] += r[e];
+            }
+            store_vec<T, VEC>((T*)p.dx + row * H + c, H - c, o);
+        }
+    }
+    // the workgroup's rows together, in a fixed order; the partial sums are added up by rms_dgamma_kernel (no atomics: the same call gives the same bits)
+#pragma unroll
+    for (int i = 0; i < NS; ++i) {
+        const int c = i * SLAB + c0;
+        if constexpr (RPB > 1) {
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) gred[wave][lane * VEC + e] = dg[i][e];
+            __syncthreads();
+            for (int k = threadIdx.x; k < SLAB; k += 256)
+                if (i * SLAB + k < H) {
+                    float s = 0.f;
+#pragma unroll
+                    for (int w = 0; w < RPB; ++w) s += gred[w][k];
+                    p.part[(int64_t)blockIdx.x * H + i * SLAB + k] = s;
+                }
+        } else {
+            store_vec<float, VEC>(p.part + (int64_t)blockIdx.x * H + c, H - c, dg[i]);
+        }
+    }
+}
+
+// dgamma[c] += sum over the nb partial rows, 64 columns x 16 row groups per workgroup
+__global__ __launch_bounds__(1024) void rms_dgamma_kernel(const float* __restrict__ part, float* __restrict__ dgamma, int nb, int H) {
+    __shared__ float red[16][64];
+    const int col = blockIdx.x * 64 + (threadIdx.x & 63), grp = threadIdx.x >> 6;
+    float s = 0.f;
+    if (col < H) {
+#pragma unroll 8
+        for (int r = grp; r < nb; r += 16) s += part[(int64_t)r * H + col];
+    }
+    red[grp][threadIdx.x & 63] = s;
+    __syncthreads();
+    if (grp == 0 && col < H) {
+#pragma unroll
+        for (int w = 1; w < 16; ++w) s += red[w][threadIdx.x];
+        dgamma[col] += s;
+    }
+}
+
+constexpr int RMS_MAX_H = 16384;
+
+// (VEC, NS, WPR) by width: one wave and 8 features per lane up to 2 048, but 4 per lane where 8 would leave half of the last slab's lanes idle (ceil(H / 256)
+// odd, up to 768); four waves above
+#define RMS_DISPATCH(H, CALL)                                                                                   \
+    do {                                                                                                        \
+        if ((H) <= 256) { constexpr int VEC = 4, NS = 1, WPR = 1; CALL; }                                       \
+        else if ((H) <= 512) { constexpr int VEC = 8, NS = 1, WPR = 1; CALL; }                                  \
+        else if ((H) <= 768) { constexpr int VEC = 4, NS = 3, WPR = 1; CALL; }                                  \
+        else if ((H) <= 1024) { constexpr int VEC = 8, NS = 2, WPR = 1; CALL; }                                 \
+        else if ((H) <= 2048) { constexpr int VEC = 8, NS = 4, WPR = 1; CALL; }                                 \
+        else if ((H) <= 4096) { constexpr int VEC = 8, NS = 2, WPR = 4; CALL; }                                 \
+        else if ((H) <= 8192) { constexpr int VEC = 8, NS = 4, WPR = 4; CALL; }                                 \
+        else { constexpr int VEC = 8, NS = 8, WPR = 4; CALL; }                                                  \
+    } while (0)
+
+int rms_rows_per_block(int H) { return H <= 2048 ? 4 : 1; }
+
+int rms_bwd_blocks(int64_t rows, int H) {
+    const int64_t nb = (rows + rms_rows_per_block(H) - 1) / rms_rows_per_block(H);
+    return (int)(nb < 1024 ? nb : 1024);
+}
+
+template <typename T>
+void rms_fwd_launch(const RmsFwdArgs& a, hipStream_t s) {
+    const int64_t nb = (a.rows + rms_rows_per_block(a.H) - 1) / rms_rows_per_block(a.H);
+    const dim3 grid((unsigned)(nb < 4096 ? nb : 4096)), block(256);
+    if (a.res)
+        RMS_DISPATCH(a.H, hipLaunchKernelGGL((rms_fwd_kernel<T, VEC, NS, WPR, true>), grid, block, 0, s, a));
+    else
+        RMS_DISPATCH(a.H, hipLaunchKernelGGL((rms_fwd_kernel<T, VEC, NS, WPR, false>), grid, block, 0, s, a));
+}
+
+}  // namespace
+
+extern "C" int merlot_rms_fwd(const void* x, int64_t ldx, int x_f32, const void* residual, int64_t ldr, const float* gamma, void* h, void* y, float* rstd,
+                              void* y8, int64_t ld8, uint8_t* scale8, int64_t ld_scale8, int64_t rows, int H, float eps, merlot_stream_t stream) {
+    MERLOT_CHECK(x && gamma && (y || y8), MERLOT_ESHAPE, "merlot_rms_fwd: null operand");
+    MERLOT_CHECK(rows > 0, MERLOT_ESHAPE, "merlot_rms_fwd: rows must be > 0");
+    MERLOT_CHECK(H > 0 && H <= RMS_MAX_H, MERLOT_ESHAPE, "merlot_rms_fwd: H=%d unsupported (1 ... %d)", H, RMS_MAX_H);
+    MERLOT_CHECK(ldx >= H && (!residual || ldr >= H), MERLOT_ESHAPE, "merlot_rms_fwd: row stride smaller than H");
+    MERLOT_CHECK((residual != nullptr) == (h != nullptr), MERLOT_ESHAPE, "merlot_rms_fwd: h is written with a residual, and only then");
+    const int64_t Hp = (H + 127) / 128 * 128;
+    MERLOT_CHECK(!y8 || (scale8 && ld8 == Hp && ld_scale8 >= Hp / 128), MERLOT_ESHAPE, "merlot_rms_fwd: the 8-bit copy has ceil(H / 128) * 128 columns and a scale per 128");
+    MERLOT_CHECK(!y8 || ((uintptr_t)y8 & 7) == 0, MERLOT_EALIGN, "merlot_rms_fwd: the 8-bit copy must be 8-byte aligned");
+    const RmsFwdArgs a = {x, ldx, residual, ldr, gamma, h, y, rstd, (uint8_t*)y8, Hp, scale8, ld_scale8, rows, H, eps};
+    if (x_f32) rms_fwd_launch<float>(a, (hipStream_t)stream);
+    else rms_fwd_launch<bf16>(a, (hipStream_t)stream);
+    return merlot_launch_status("merlot_rms_fwd");
+}
+
+extern "C" int64_t merlot_rms_bwd_workspace_bytes(int64_t rows, int H) {
+    if (rows <= 0 || H <= 0 || H > RMS_MAX_H) return 0;
+    return (int64_t)rms_bwd_blocks(rows, H) * H * 4;
+}
+
+extern "C" int merlot_rms_bwd(const void* dy, int64_t lddy, int is_f32, const void* h, int64_t ldh, const float* rstd, const float* gamma, const void* dres,
+                              int64_t lddr, void* dx, float* dgamma, int64_t rows, int H, void* workspace, int64_t workspace_bytes, merlot_stream_t stream) {
+    MERLOT_CHECK(dy && h && rstd && gamma && dx && dgamma, MERLOT_ESHAPE, "merlot_rms_bwd: null operand");
+    MERLOT_CHECK(rows > 0, MERLOT_ESHAPE, "merlot_rms_bwd: rows must be > 0");
+    MERLOT_CHECK(H > 0 && H <= RMS_MAX_H, MERLOT_ESHAPE, "merlot_rms_bwd: H=%d unsupported (1 ... %d)", H, RMS_MAX_H);
+    MERLOT_CHECK(lddy >= H && ldh >= H && (!dres || lddr >= H), MERLOT_ESHAPE, "merlot_rms_bwd: row stride smaller than H");
+    MERLOT_CHECK(workspace && workspace_bytes >= merlot_rms_bwd_workspace_bytes(rows, H), MERLOT_ESHAPE, "merlot_rms_bwd: workspace too small");
+    const int nb = rms_bwd_blocks(rows, H);
+    const RmsBwdArgs a = {dy, lddy, h, ldh, rstd, gamma, dres, lddr, dx, (float*)workspace, rows, H};
+    hipStream_t s = (hipStream_t)stream;
+    const dim3 grid(nb), block(256);
+    if (is_f32) RMS_DISPATCH(H, hipLaunchKernelGGL((rms_bwd_kernel<float, VEC, NS, WPR>), grid, block, 0, s, a));
+    else RMS_DISPATCH(H, hipLaunchKernelGGL((rms_bwd_kernel<bf16, VEC, NS, WPR>), grid, block, 0, s, a));
+    if (int rc = merlot_launch_status("merlot_rms_bwd")) return rc;
+    hipLaunchKernelGGL(rms_dgamma_kernel, dim3((H + 63) / 64), dim3(1024), 0, s, (const float*)workspace, dgamma, nb, H);
+    return merlot_launch_status("merlot_rms_bwd");
+}

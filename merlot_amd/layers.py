@@ -565,6 +565,85 @@ def layer_norm(x, ln, out_bf16=False):
     return LayerNormFn.apply(x, ln, out_bf16)
 
 
+class RMSNormFn(torch.autograd.Function):
+    """y = h / rms(h) * gamma with h = x (+ residual); outputs y, or (y, h) with a residual: h is the residual stream behind the addition."""
+
+    @staticmethod
+    def forward(ctx, x, residual, norm, eps):
+        ctx.set_materialize_grads(False)
+        y, h, rstd, _, _ = ops.rms_norm_fwd(x, norm.gamma, residual=residual, eps=eps)
+        ctx.norm, ctx.rstd, ctx.two = norm, rstd, residual is not None
+        ctx.save_for_backward(h if ctx.two else x)
+        return (y, h) if ctx.two else y
+
+    @staticmethod
+    def backward(ctx, dy, dh=None):
+        if dy is None:                                   # only the residual stream is used downstream: the addition alone
+            return dh, dh if ctx.two else None, None, None
+        h, = ctx.saved_tensors
+        dx = ops.rms_norm_bwd(dy.contiguous(), h, ctx.rstd, ctx.norm.gamma, ctx.norm.ggamma, dres=None if dh is None else dh.contiguous())
+        return dx, dx if ctx.two else None, None, None
+
+
+def rms_norm(x, norm, residual=None, eps=1e-6):
+    """root-mean-square norm over the last dimension with the gain of `norm` (a ParamStore.ln handle: gamma, and ggamma, which the backward ACCUMULATES into).
+    x bf16 or f32 [..., H]; with a residual of the same type and shape: -> (y, h = x + residual), both differentiable."""
+    return RMSNormFn.apply(x, residual, norm, eps)
+
+
+def _w8_blocks(lin):
+    """the 8-bit copies of a Linear's bf16 working weight, both orientations in 128 x 128 tiles: made once per version of the working copies and stream (they change
+    at the optimizer step only).  A captured launch makes its own: a replay has to see the weights of ITS time.  A new version gets new tensors, so a backward
+    that is still to come keeps the copies its forward used."""
+    store = lin._store
+    if store is None or torch.cuda.is_current_stream_capturing():
+        return ops.quantize_blocks(lin.wb, tile=128, transpose=True)
+    cache = store.__dict__.setdefault('_w8_blocks', {})
+    key = (lin.name, torch.cuda.current_stream().cuda_stream)
+    ent = cache.get(key)
+    if ent is None or ent[0] != store.version:
+        ent = cache[key] = (store.version, ops.quantize_blocks(lin.wb, tile=128, transpose=True))
+    return ent[1]
+
+
+class LinearF8BlocksFn(torch.autograd.Function):
+    """y = x W^T + b with all three products of the layer on 8-bit blocks (ops.gemm_f8_blocks).  x is quantised once, row-wise for this product and transposed for
+    the weight gradient: what waits for the backward is the one-byte transposed copy, not x."""
+
+    @staticmethod
+    def forward(ctx, x, lin, grad_fmt):
+        if lin.gb is not None and lin.w.shape[0] % 4 != 0:
+            raise ValueError("linear_f8_blocks: a Linear with a bias needs an output width that is a multiple of 4 (the bias gradient's column sums)")
+        x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+        w8, sw, wt8, swt = _w8_blocks(lin)
+        if ctx.needs_input_grad[0]:
+            x8, sx, xt8, sxt = ops.quantize_blocks(x2, transpose=True)
+        else:
+            (x8, sx), xt8, sxt = ops.quantize_blocks(x2), None, None
+        ctx.lin, ctx.grad_fmt, ctx.shape, ctx.dtype = lin, grad_fmt, x.shape, x.dtype
+        ctx.save_for_backward(xt8, sxt, wt8, swt)
+        return ops.gemm_f8_blocks(x8, sx, w8, sw, bias=lin.b).view(*x.shape[:-1], lin.w.shape[0])
+
+    @staticmethod
+    def backward(ctx, dy):
+        lin = ctx.lin
+        xt8, sxt, wt8, swt = ctx.saved_tensors
+        dy2 = dy.contiguous().view(-1, dy.shape[-1])
+        if dy2.shape[0] == 0:
+            return torch.zeros(ctx.shape, device=dy.device, dtype=ctx.dtype), None, None
+        d8, sd, dt8, sdt = ops.quantize_blocks(dy2, ctx.grad_fmt, transpose=True)
+        ops.gemm_f8_blocks(dt8, sdt, xt8, sxt, out=lin.gw, accumulate=True)
+        if lin.gb is not None:
+            ops.colsum_bf16(dy2, lin.gb)
+        return ops.gemm_f8_blocks(d8, sd, wt8, swt, out_dtype=ctx.dtype).view(ctx.shape), None, None
+
+
+def linear_f8_blocks(x, lin, grad_fmt=ops.F8_E4M3):
+    """x [..., in] (bf16 or f32) -> bf16 [..., out]; weight and bias gradients are ACCUMULATED into the Linear's gradient views.  Operands are e4m3 with a scale per
+    128 values along each product's reduction (activations) or per 128 x 128 tile (weights); grad_fmt: the format of dy."""
+    return LinearF8BlocksFn.apply(x, lin, grad_fmt)
+
+
 class GatherAddFn(torch.autograd.Function):
     """out[r] = sum_k table_k[idx_k[r]]   (f32).  `act` (optional) is an activation tensor source (bf16 or f32,
     differentiable through autograd); tables are (param, grad, idx[, period]) tuples from the store, gradients

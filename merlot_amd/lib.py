@@ -14,7 +14,7 @@ LIB_PATH = os.path.join(_HERE, 'libmerlot_hip.so')
 _CTYPES = {
     'const void*': ctypes.c_void_p, 'void*': ctypes.c_void_p,
     'const float*': ctypes.c_void_p, 'float*': ctypes.c_void_p,
-    'const int32_t*': ctypes.c_void_p, 'int32_t*': ctypes.c_void_p, 'int64_t*': ctypes.c_void_p,
+    'const int32_t*': ctypes.c_void_p, 'int32_t*': ctypes.c_void_p, 'int64_t*': ctypes.c_void_p, 'const int64_t*': ctypes.c_void_p,
     'const uint8_t*': ctypes.c_void_p, 'uint8_t*': ctypes.c_void_p, 'const merlot_image_job_t*': ctypes.c_void_p,
     'const int16_t*': ctypes.c_void_p, 'int16_t*': ctypes.c_void_p,
     'const merlot_jpeg_info_t*': ctypes.c_void_p, 'merlot_jpeg_info_t*': ctypes.c_void_p,

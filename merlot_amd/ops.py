@@ -897,3 +897,247 @@ def weight_std_bwd(dkhat_t, khat, rstd, gk2d):
     assert gk2d.is_contiguous() and khat.is_contiguous()
     K, Co = khat.shape
     call('merlot_weight_std_bwd', _p(dkhat_t), dkhat_t.stride(0), _p(khat), _p(rstd), K, Co, _p(gk2d), _stream())
+
+
+# ---- root-mean-square norm, 8-bit blocks, gradient clipping ------------------------------------------------------------------
+def _here(*tensors):
+    """every tensor on the CURRENT device (the library launches on the current device's stream)"""
+    dev = torch.cuda.current_device()
+    for t in tensors:
+        if t is not None and t.is_cuda and t.device.index != dev:
+            raise ValueError(f"a tensor on {t.device} while the current device is cuda:{dev}: call under torch.cuda.device({t.device.index})")
+
+
+def _rows(t, name):
+    """(2-D view, row stride): any leading dims where they collapse without a copy; rows may be further apart than they are long, not nearer"""
+    if t.dim() == 0:
+        raise ValueError(f"{name}: expected at least one dimension")
+    if t.dim() != 2:
+        try:
+            t = t.view(-1, t.shape[-1]) if t.numel() else t.reshape(0, t.shape[-1])
+        except RuntimeError:
+            raise ValueError(f"{name}: leading dimensions do not collapse into rows without a copy") from None
+    if t.shape[0] <= 1:
+        return t, t.shape[1]
+    if t.stride(0) < t.shape[1]:
+        raise ValueError(f"{name}: rows overlap (stride {t.stride(0)}, {t.shape[1]} columns)")
+    return t, t.stride(0)
+
+
+def _scales8(rows, cols, device):
+    """scale bytes of `rows` rows of `cols` values, a byte per block of 128; rows 4-byte aligned (the product reads them as words)"""
+    nb = (cols + 127) // 128
+    return torch.empty((rows, (nb + 3) // 4 * 4), device=device, dtype=torch.uint8)[:, :nb]
+
+
+def rms_norm_fwd(x, gamma, *, residual=None, out=True, q8=False, save_rstd=True, eps=1e-6):
+    """h = x + residual (rounded to x's type), R = 1 / sqrt(mean(h^2) + eps), y = h * R * gamma over the last dimension (1 ... 16 384 features).
+    x [..., H] bf16 or f32, residual like x (or None: h is x), gamma f32 [H].  -> (y, h, rstd, y8, scale8): y like x (None: out False); h None without a
+    residual; rstd f32 [rows] (None: save_rstd False); q8: y8 / scale8 = the e4m3 copy of the unrounded y in blocks of 128 features, as quantize_blocks
+    lays it out -- the left operand of gemm_f8_blocks."""
+    if x.dtype not in (BF16, F32):
+        raise ValueError(f"x: expected bf16 or f32, got {x.dtype}")
+    _chk(x, x.dtype, 'x'); _chk(gamma, F32, 'gamma'); _chk(residual, x.dtype, 'residual'); _here(x, gamma, residual)
+    x2, ldx = _rows(x, 'x')
+    rows, H = x2.shape
+    if gamma.shape != (H,):
+        raise ValueError(f"gamma: expected [{H}], got {tuple(gamma.shape)}")
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"residual: expected {tuple(x.shape)}, got {tuple(residual.shape)}")
+    if not out and not q8:
+        raise ValueError("rms_norm_fwd: neither out nor q8 is asked for")
+    r2, ldr = _rows(residual, 'residual') if residual is not None else (None, 0)
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype) if out else None
+    h = torch.empty(x.shape, device=x.device, dtype=x.dtype) if residual is not None else None
+    rstd = torch.empty(rows, device=x.device, dtype=F32) if save_rstd else None
+    y8 = s8 = None
+    if q8:
+        y8 = torch.empty((rows, (H + 127) // 128 * 128), device=x.device, dtype=FP8)
+        s8 = _scales8(rows, H, x.device)
+    if rows:
+        call('merlot_rms_fwd', _p(x2), ldx, 1 if x.dtype == F32 else 0, _p(r2), ldr, _p(gamma), _p(h), _p(y), _p(rstd), _p(y8), y8.shape[1] if q8 else 0,
+             _p(s8), (s8.shape[1] + 3) // 4 * 4 if q8 else 0, rows, H, float(eps), _stream())
+    return y, h, rstd, y8, s8
+
+
+def rms_norm_bwd(dy, h, rstd, gamma, dgamma, *, dres=None):
+    """gradient of rms_norm_fwd: h (x where there was no residual) and rstd as the forward left them, dy the gradient of y, dres that of h from elsewhere (the
+    residual stream).  -> dx, which is the residual's gradient too; dgamma f32 [H] is ACCUMULATED, in a fixed order (the same call gives the same bits)."""
+    if h.dtype not in (BF16, F32):
+        raise ValueError(f"h: expected bf16 or f32, got {h.dtype}")
+    for t, dt, nm in ((h, h.dtype, 'h'), (dy, h.dtype, 'dy'), (dres, h.dtype, 'dres'), (rstd, F32, 'rstd'), (gamma, F32, 'gamma'), (dgamma, F32, 'dgamma')):
+        _chk(t, dt, nm)
+    _here(h, dy, dres, rstd, gamma, dgamma)
+    h2, ldh = _rows(h, 'h')
+    rows, H = h2.shape
+    for t, nm in ((dy, 'dy'), (dres, 'dres')):
+        if t is not None and t.shape != h.shape:
+            raise ValueError(f"{nm}: expected {tuple(h.shape)}, got {tuple(t.shape)}")
+    if gamma.shape != (H,) or dgamma.shape != (H,):
+        raise ValueError(f"gamma, dgamma: expected [{H}], got {tuple(gamma.shape)}, {tuple(dgamma.shape)}")
+    if rstd.numel() != rows or not rstd.is_contiguous():
+        raise ValueError(f"rstd: expected {rows} dense values")
+    dy2, lddy = _rows(dy, 'dy')
+    dr2, lddr = _rows(dres, 'dres') if dres is not None else (None, 0)
+    dx = torch.empty(h.shape, device=h.device, dtype=h.dtype)
+    if rows:
+        nbytes = LIB.query('merlot_rms_bwd_workspace_bytes', rows, H)
+        ws = torch.empty(nbytes // 4, device=h.device, dtype=F32)
+        call('merlot_rms_bwd', _p(dy2), lddy, 1 if h.dtype == F32 else 0, _p(h2), ldh, _p(rstd), _p(gamma), _p(dr2), lddr, _p(dx), _p(dgamma), rows, H,
+             _p(ws), nbytes, _stream())
+    return dx
+
+
+def quantize_blocks(x, fmt=F8_E4M3, *, tile=1, rows=True, transpose=False):
+    """8-bit copies of x [R, C] (bf16 or f32) with a power-of-two scale for each block of 128 -> (q, s), or (q, s, qt, st) with transpose (rows=False: q, s None).
+    q [R, C padded with zeros to whole blocks] float8, s [R, blocks] uint8: a byte b stands for 2^(b - 127), the least power of two that brings the block's max |x|
+    to the format's largest value or under it; 255 = NaN, for a block that holds an infinity or NaN.  qt / st: the same of x^T, blocks along x's rows.
+    tile=128: one scale per 128 x 128 tile (weights: q and qt then hold the same values).  fmt: F8_E4M3 or F8_E5M2."""
+    if x.dtype not in (BF16, F32):
+        raise ValueError(f"x: expected bf16 or f32, got {x.dtype}")
+    _chk(x, x.dtype, 'x'); _here(x)
+    if x.dim() != 2 or x.shape[1] == 0:
+        raise ValueError(f"x: expected [rows, columns >= 1], got {tuple(x.shape)}")
+    if fmt not in _F8_DTYPES or tile not in (1, 128):
+        raise ValueError("quantize_blocks: fmt must be F8_E4M3 or F8_E5M2, tile 1 or 128")
+    if not rows and not transpose:
+        raise ValueError("quantize_blocks: neither rows nor transpose is asked for")
+    x2, ldx = _rows(x, 'x')
+    R, C = x.shape
+    dt = _F8_DTYPES[fmt]
+    q = s = qt = st = None
+    if rows:
+        q, s = torch.empty((R, (C + 127) // 128 * 128), device=x.device, dtype=dt), _scales8(R, C, x.device)
+    if transpose:
+        qt, st = torch.empty((C, (R + 127) // 128 * 128), device=x.device, dtype=dt), _scales8(C, R, x.device)
+    if R:
+        call('merlot_quantize_blocks', _p(x2), ldx, 1 if x.dtype == F32 else 0, R, C, int(fmt), int(tile), _p(q), q.shape[1] if rows else 0, _p(s),
+             (s.shape[1] + 3) // 4 * 4 if rows else 0, _p(qt), qt.shape[1] if transpose else 0, _p(st), (st.shape[1] + 3) // 4 * 4 if transpose else 0, _stream())
+    return (q, s, qt, st) if transpose else (q, s)
+
+
+def _scale_ld(s, rows, nb, name):
+    _chk(s, torch.uint8, name)
+    if s.shape != (rows, nb):
+        raise ValueError(f"{name}: expected [{rows}, {nb}] scale bytes, got {tuple(s.shape)}")
+    ld = (nb + 3) // 4 * 4 if rows <= 1 else s.stride(0)
+    if rows and s.storage_offset() + (rows - 1) * ld + (nb + 3) // 4 * 4 > s.untyped_storage().nbytes():
+        raise ValueError(f"{name}: rows are read in whole words of 4 bytes, the last one ends before its word does")
+    return ld
+
+
+def gemm_f8_blocks(a8, a_scale, b8, b_scale, *, bias=None, out=None, out_dtype=BF16, accumulate=False):
+    """C[M,N] (+)= a8[M,K] @ b8[N,K]^T (+ bias) on 8-bit operands with a scale per row and block of 128, as quantize_blocks / rms_norm_fwd(q8=True) make them: a8 e4m3
+    or e5m2, b8 e4m3, K a multiple of 128; M, N any.  fp32 accumulation; C bf16 or f32 (out / out_dtype), accumulate (f32 out only) adds into out."""
+    fa = 1 if a8.dtype == torch.float8_e5m2 else 0
+    _chk(a8, _F8_DTYPES[fa], 'a8'); _chk(b8, FP8, 'b8'); _chk(bias, F32, 'bias'); _here(a8, a_scale, b8, b_scale, bias, out)
+    if a8.dim() != 2 or b8.dim() != 2 or a8.shape[1] != b8.shape[1] or a8.shape[1] == 0 or a8.shape[1] % 128 != 0:
+        raise ValueError(f"gemm_f8_blocks: operands [M, K] and [N, K] with K a multiple of 128, got {tuple(a8.shape)} and {tuple(b8.shape)}")
+    M, K = a8.shape
+    N = b8.shape[0]
+    _, lda = _rows(a8, 'a8')
+    _, ldb = _rows(b8, 'b8')
+    ldsa, ldsb = _scale_ld(a_scale, M, K // 128, 'a_scale'), _scale_ld(b_scale, N, K // 128, 'b_scale')
+    if bias is not None and bias.shape != (N,):
+        raise ValueError(f"bias: expected [{N}], got {tuple(bias.shape)}")
+    if out is None:
+        if accumulate:
+            raise ValueError("gemm_f8_blocks: accumulate needs out")
+        if out_dtype not in (BF16, F32):
+            raise ValueError(f"out_dtype: expected bf16 or f32, got {out_dtype}")
+        out = torch.empty((M, N), device=a8.device, dtype=out_dtype)
+    if out.dtype not in (BF16, F32) or out.shape != (M, N):
+        raise ValueError(f"out: expected bf16 or f32 [{M}, {N}], got {out.dtype} {tuple(out.shape)}")
+    if accumulate and out.dtype != F32:
+        raise ValueError("gemm_f8_blocks: accumulate needs an f32 out")
+    if M == 0 or N == 0:
+        return out
+    _chk(out, out.dtype, 'out')
+    _, ldc = _rows(out, 'out')
+    nbytes = LIB.query('merlot_gemm_f8_blocks_workspace_bytes', M, N, K)
+    ws = torch.empty(nbytes // 4, device=a8.device, dtype=F32) if nbytes else None   # caller-owned partial products of a split reduction
+
+    def launch():
+        call('merlot_gemm_f8_blocks', _p(a8), lda, fa, _p(a_scale), ldsa, _p(b8), ldb, _p(b_scale), ldsb, _p(out), ldc, M, N, K, 1 if out.dtype == F32 else 0,
+             1 if accumulate else 0, _p(bias), _p(ws), nbytes, _stream())
+
+    if TIMER is not None:
+        TIMER.time('gemm_f8_blocks', 2.0 * M * N * K, launch)
+    else:
+        launch()
+    return out
+
+
+class TensorList(object):
+    """Many dense f32 / bf16 tensors of one device as ONE operand (global_norm, clip_by_global_norm): checked once, for as long as the tensors stay where they are.
+    Holds references to them; a tensor whose storage has been exchanged since (`t.data = ...`) makes the next use raise."""
+
+    def __init__(self, tensors):
+        import ctypes
+        self.tensors = tuple(tensors)
+        n = len(self.tensors)
+        if n == 0:
+            raise ValueError("TensorList: no tensors")
+        dev = self.tensors[0].device
+        for i, t in enumerate(self.tensors):
+            if not t.is_cuda or t.device != dev:
+                raise ValueError(f"tensor {i}: expected a GPU tensor on {dev}, got {t.device}")
+            if t.dtype not in (F32, BF16):
+                raise ValueError(f"tensor {i}: expected f32 or bf16, got {t.dtype}")
+            if not t.is_contiguous():
+                raise ValueError(f"tensor {i}: must be contiguous")
+        self.device = dev
+        self.shapes = [t.shape for t in self.tensors]
+        self.addresses = [t.data_ptr() for t in self.tensors]
+        self.ptrs = (ctypes.c_int64 * n)(*self.addresses)
+        self.numels = (ctypes.c_int64 * n)(*[t.numel() for t in self.tensors])
+        self.bf16 = bytes(1 if t.dtype == BF16 else 0 for t in self.tensors)
+
+    def __len__(self):
+        return len(self.tensors)
+
+    def check(self):
+        if [t.data_ptr() for t in self.tensors] != self.addresses or [t.shape for t in self.tensors] != self.shapes:
+            raise ValueError("TensorList: a tensor's storage or shape has changed since the list was made")
+
+
+def _tensor_list(ts):
+    if not isinstance(ts, TensorList):
+        return TensorList(ts)
+    ts.check()
+    return ts
+
+
+def _clip(grads, clip, out):
+    import ctypes
+    types = bytes(a | (b << 1) for a, b in zip(grads.bf16, out.bf16))
+    _here(grads.tensors[0], out.tensors[0])
+    n = len(grads)
+    norm = torch.empty((), device=grads.device, dtype=F32)
+    nbytes = LIB.query('merlot_clip_workspace_bytes', n)
+    ws = torch.empty(nbytes // 8, device=grads.device, dtype=torch.float64)
+    call('merlot_clip_by_global_norm', ctypes.addressof(grads.ptrs), ctypes.addressof(out.ptrs), ctypes.addressof(grads.numels), ctypes.cast(types, ctypes.c_void_p),
+         n, float(clip), _p(norm), _p(ws), nbytes, _stream())
+    return norm
+
+
+def global_norm(grads):
+    """sqrt of the sum of squares over all elements of all tensors (a list, or a TensorList), summed in 64 bits -> f32 scalar on the device."""
+    grads = _tensor_list(grads)
+    return _clip(grads, 0.0, grads)
+
+
+def clip_by_global_norm(grads, clip_norm, out=None):
+    """every tensor times clip_norm / max(norm, clip_norm), norm = global_norm(grads); in place, or into `out` (tensors of the same shapes, f32 or bf16 each, that
+    share no memory with each other or with other inputs).  grads, out: lists, or TensorLists a program keeps.  -> the norm BEFORE clipping (f32 scalar on the
+    device).  An infinite norm scales by 0, a NaN one makes every element NaN."""
+    clip_norm = float(clip_norm)
+    if not 0.0 < clip_norm < float('inf'):
+        raise ValueError(f"clip_norm: expected a positive finite number, got {clip_norm}")
+    grads = _tensor_list(grads)
+    out = grads if out is None else _tensor_list(out)
+    if out.shapes != grads.shapes:
+        raise ValueError("clip_by_global_norm: out must hold tensors of the same shapes as grads")
+    if out.device != grads.device:
+        raise ValueError(f"clip_by_global_norm: out is on {out.device}, grads on {grads.device}")
+    return _clip(grads, clip_norm, out)
