@@ -23,6 +23,7 @@ struct BlocksArgs {
     int nk, nk_split;                        // blocks of 128 in all, per split
     int ntm, ntn;
     int accumulate;
+    unsigned band_magic;                     // 2^32 / (4 ntn): blocks_wide_kernel
 };
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint8_t* p, int64_t row0, int64_t rows, int64_t ld, int64_t width) {
@@ -30,11 +31,10 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint8_t* p, in
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p + row0 * ld), 0, rows > 0 ? (int)((rows - 1) * ld + width) : 0, 0x00020000);
 }
 
-// up to E consecutive columns n ... of row m; add: onto what is there (fp32 only)
+// up to E consecutive columns at c, `left` of which exist; add: onto what is there (fp32 only)
 template <typename T, int E>
-__device__ __forceinline__ void store_out(T* C, int64_t ldc, int64_t m, int64_t n, int64_t left, T __attribute__((ext_vector_type(E))) v, bool add) {
+__device__ __forceinline__ void store_out(T* c, int64_t left, T __attribute__((ext_vector_type(E))) v, bool add) {
     typedef T vec_t __attribute__((ext_vector_type(E), aligned(sizeof(T))));
-    T* c = C + m * ldc + n;
     if (left >= E) {
         if constexpr (sizeof(T) == 4)
             if (add) v += *reinterpret_cast<const vec_t*>(c);
@@ -70,8 +70,8 @@ __device__ __forceinline__ bf16x8 widen(int lo, int hi, float scale) {
 template <int N>
 __device__ __forceinline__ void wait_step() { asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory"); }
 
-// Tile 128 x BN, four waves (64 x 128 each for BN 256, 64 x 64 for BN 128), K-steps of 64, three step buffers filled by LDS-DMA two steps ahead, one barrier per
-// step.  Two workgroups share a CU (72 + 6 KiB of LDS, 256 registers): while one waits, loads or stores its tile, the other multiplies.
+// Tile 128 x BN, four waves (64 x 128 each for BN 256, 64 x 64 for BN 128), K-steps of 64, three step buffers filled by LDS-DMA two to three steps ahead, one
+// barrier per step.  Two workgroups share a CU (72 + 6 KiB of LDS, 256 registers): while one waits, loads or stores its tile, the other multiplies.
 // OUT: 0 bf16, 1 fp32, 2 fp32 partial products of a split reduction.  EXACT: through bf16 fragments (see above).
 constexpr int SCALE_BLOCKS = 16;                         // blocks of 128 whose scale bytes lie in LDS at a time (16 bytes per row)
 
@@ -108,11 +108,11 @@ __global__ __launch_bounds__(256, 2) void blocks_gemm_kernel(const BlocksArgs p)
         const int row = (i < 2 ? wave * 2 + i : wave * (PIECES - 2) + i - 2) * 16 + (lane >> 2), ch = ((lane & 3) ^ (row >> 2)) & 3;
         off[i] = (unsigned)(row * (i < 2 ? p.lda : p.ldb)) + ch * 16;
     }
-    auto issue = [&](int step, int buf) {
+    auto issue = [&](int step, int base) {       // base: byte offset of the buffer
 #pragma unroll
         for (int i = 0; i < PIECES; ++i) {
-            if (i < 2) __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, LDS_PTR(lds + buf * STEP + (wave * 2 + i) * 1024), 16, off[i], step * 64, 0, 0);
-            else __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, LDS_PTR(lds + buf * STEP + (8 + wave * (PIECES - 2) + i - 2) * 1024), 16, off[i], step * 64, 0, 0);
+            if (i < 2) __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, LDS_PTR(lds + base + (wave * 2 + i) * 1024), 16, off[i], step * 64, 0, 0);
+            else __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, LDS_PTR(lds + base + (8 + wave * (PIECES - 2) + i - 2) * 1024), 16, off[i], step * 64, 0, 0);
         }
     };
     // the scale bytes of sixteen blocks from block b on, a word of four blocks per thread and turn (a split starts at a multiple of four blocks)
@@ -148,60 +148,101 @@ __global__ __launch_bounds__(256, 2) void blocks_gemm_kernel(const BlocksArgs p)
         rb_off[j] = row * 64;
         cb[j] = ((2 * hi) ^ (row >> 2)) & 3;
     }
-    auto fragment = [&](int buf, unsigned row_off, unsigned c) -> i32x8 {
-        const i32x4 x = *reinterpret_cast<const i32x4*>(lds + buf * STEP + row_off + c * 16);
-        const i32x4 y = *reinterpret_cast<const i32x4*>(lds + buf * STEP + row_off + (c ^ 1) * 16);
+    auto fragment = [&](int base, unsigned row_off, unsigned c) -> i32x8 {
+        const i32x4 x = *reinterpret_cast<const i32x4*>(lds + base + row_off + c * 16);
+        const i32x4 y = *reinterpret_cast<const i32x4*>(lds + base + row_off + (c ^ 1) * 16);
         return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
     };
+    // One step = two halves of the wave's columns.  The second half's B fragments are read while the first half multiplies, the NEXT step's A and first-half B
+    // fragments while the second half does; the barrier stands between the halves: behind it the step's buffer is free (every read of it has returned) and takes
+    // step t + 3, and step t + 1 is complete.
     const int steps = 2 * (kb1 - kb0);
+    constexpr int NH = NJ / 2;
     issue(2 * kb0, 0);
-    issue(2 * kb0 + 1, 1);
-    int buf = 0;
+    issue(2 * kb0 + 1, STEP);
+    if (steps > 2) { issue(2 * kb0 + 2, 2 * STEP); wait_step<2 * PIECES>(); }
+    else wait_step<PIECES>();
+    __builtin_amdgcn_s_barrier();
+    i32x8 fa[2][2], fb0[NH], fb1[NH];                    // fa: [parity of the step]
     int xa[2], xb[NJ];
-    for (int t = 0; t < steps; ++t) {
-        // the last words of the old sixteen blocks were read eight steps ago, seven barriers back
-        if (t && (t & (2 * SCALE_BLOCKS - 1)) == 0) load_scales(kb0 + (t >> 1));
-        if (t + 1 < steps) wait_step<PIECES>();
-        else wait_step<0>();
-        __builtin_amdgcn_s_barrier();
-        if (t + 2 < steps) issue(2 * kb0 + t + 2, buf == 0 ? 2 : buf - 1);
-        if ((t & 7) == 0) {                              // four blocks' bytes per word
+    auto read_scales = [&](int w) {                      // a word holds four blocks' bytes
 #pragma unroll
-            for (int i = 0; i < 2; ++i) xa[i] = *reinterpret_cast<const int*>(scales + (wm * 64 + i * 32 + l31) * 16 + ((t >> 3) & 3) * 4);
+        for (int i = 0; i < 2; ++i) xa[i] = *reinterpret_cast<const int*>(scales + (wm * 64 + i * 32 + l31) * 16 + w * 4);
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) xb[j] = *reinterpret_cast<const int*>(scales + (BM + wn * (BN / 2) + j * 32 + l31) * 16 + ((t >> 3) & 3) * 4);
-        } else if ((t & 1) == 0) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) xa[i] = (int)((unsigned)xa[i] >> 8);
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) xb[j] = (int)((unsigned)xb[j] >> 8);
-        }
-        i32x8 fa[2], fb[NJ];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) fa[i] = fragment(buf, ra_off[i], ca[i]);
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) fb[j] = fragment(buf, rb_off[j], cb[j]);
+        for (int j = 0; j < NJ; ++j) xb[j] = *reinterpret_cast<const int*>(scales + (BM + wn * (BN / 2) + j * 32 + l31) * 16 + w * 4);
+    };
+    auto multiply = [&](const i32x8 (&a)[2], const i32x8 (&b)[NH], auto first) {
+        constexpr int J0 = decltype(first)::value;
         if constexpr (!EXACT) {
 #pragma unroll
-            for (int j = 0; j < NJ; ++j)
+            for (int j = 0; j < NH; ++j)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(fb[j], fa[i], acc[i][j], 0, FA, 0, xb[j], 0, xa[i]);
+                    acc[i][J0 + j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(b[j], a[i], acc[i][J0 + j], 0, FA, 0, xb[J0 + j], 0, xa[i]);
         } else {
 #pragma unroll
             for (int q = 0; q < 4; ++q) {                // lane k-bytes 8 q ... : the same eight of both operands, which is all a dot product asks for
-                bf16x8 wa[2], wb[NJ];
+                bf16x8 wa[2], wb[NH];
 #pragma unroll
-                for (int i = 0; i < 2; ++i) wa[i] = widen<FA>(fa[i][2 * q], fa[i][2 * q + 1], scale_value(xa[i] & 255));
+                for (int i = 0; i < 2; ++i) wa[i] = widen<FA>(a[i][2 * q], a[i][2 * q + 1], scale_value(xa[i] & 255));
 #pragma unroll
-                for (int j = 0; j < NJ; ++j) wb[j] = widen<0>(fb[j][2 * q], fb[j][2 * q + 1], scale_value(xb[j] & 255));
+                for (int j = 0; j < NH; ++j) wb[j] = widen<0>(b[j][2 * q], b[j][2 * q + 1], scale_value(xb[J0 + j] & 255));
 #pragma unroll
-                for (int j = 0; j < NJ; ++j)
+                for (int j = 0; j < NH; ++j)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) acc[i][j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[j], wa[i], acc[i][j], 0, 0, 0);
+                    for (int i = 0; i < 2; ++i) acc[i][J0 + j] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[j], wa[i], acc[i][J0 + j], 0, 0, 0);
             }
         }
-        buf = buf == 2 ? 0 : buf + 1;
+        // a use of the sums in this segment: without one the compiler sinks the (side-effect free) matrix instructions behind the reads they are meant to cover
+#pragma unroll
+        for (int j = 0; j < NH; ++j)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                f32x16& s = acc[i][J0 + j];
+                asm volatile("" : "+v"(s));
+            }
+    };
+    read_scales(0);
+    int cur = 0;                                         // byte offset of step t's buffer
+#pragma unroll
+    for (int i = 0; i < 2; ++i) fa[0][i] = fragment(cur, ra_off[i], ca[i]);
+#pragma unroll
+    for (int j = 0; j < NH; ++j) fb0[j] = fragment(cur, rb_off[j], cb[j]);
+    auto step = [&](int t, auto parity) {
+        constexpr int P = decltype(parity)::value;
+#pragma unroll
+        for (int j = 0; j < NH; ++j) fb1[j] = fragment(cur, rb_off[NH + j], cb[NH + j]);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(fa[P], fb0, std::integral_constant<int, 0>{});
+        __builtin_amdgcn_sched_barrier(0);
+        // the last words of the old sixteen blocks were read eight steps ago, seven barriers back
+        if (((t + 1) & (2 * SCALE_BLOCKS - 1)) == 0 && t + 1 < steps) load_scales(kb0 + ((t + 1) >> 1));
+        if (t + 2 < steps) wait_step<PIECES>();
+        else wait_step<0>();
+        __builtin_amdgcn_s_barrier();
+        if (t + 3 < steps) issue(2 * kb0 + t + 3, cur);
+        cur = cur == 2 * STEP ? 0 : cur + STEP;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) fa[P ^ 1][i] = fragment(cur, ra_off[i], ca[i]);      // (behind the last step: bytes nobody uses)
+#pragma unroll
+        for (int j = 0; j < NH; ++j) fb0[j] = fragment(cur, rb_off[j], cb[j]);
+        __builtin_amdgcn_sched_barrier(0);
+        multiply(fa[P], fb1, std::integral_constant<int, NH>{});
+        __builtin_amdgcn_sched_barrier(0);
+        if (P) {                                         // both steps of a block are done: the next byte
+            if (((t + 1) & 7) == 0) {
+                read_scales(((t + 1) >> 3) & 3);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) xa[i] = (int)((unsigned)xa[i] >> 8);
+#pragma unroll
+                for (int j = 0; j < NJ; ++j) xb[j] = (int)((unsigned)xb[j] >> 8);
+            }
+        }
+    };
+    for (int t = 0; t < steps; t += 2) {                 // (two steps per block: steps is even)
+        step(t, std::integral_constant<int, 0>{});
+        step(t + 1, std::integral_constant<int, 1>{});
     }
     // ---- epilogue: 32 rows at a time through a slab of the wave's own in the step buffers, so that memory sees whole rows of the wave's columns
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -230,8 +271,287 @@ __global__ __launch_bounds__(256, 2) void blocks_gemm_kernel(const BlocksArgs p)
             const int64_t m = m0 + wm * 64 + i * 32 + row;
             typedef T slab_t __attribute__((ext_vector_type(E)));
             const slab_t s = *reinterpret_cast<const slab_t*>(slab + row * LDR + (lane % LPR) * 16);
-            if (m < p.M && n < p.N) store_out<T, E>(C, ldc, m, n, p.N - n, s, OUT == 1 && p.accumulate);
+            if (m < p.M && n < p.N) store_out<T, E>(C + m * ldc + n, p.N - n, s, OUT == 1 && p.accumulate);
         }
+    }
+#endif
+}
+
+// Large outputs: 256 x 256 tiles, four waves of 128 x 128 -- ONE per SIMD, 256 accumulators each --, K-tiles of 128 (whole 128-byte lines per row, where 64-byte steps
+// ask the L2 twice per line), two K-tile buffers.  A wave's next fragments are read, and the next K-tile is fetched, between its own matrix instructions; the one barrier
+// per K-tile stands where the buffer's last reads have returned.  Persistent: workgroups walk the tiles of their XCD's band, the fetch stream runs on across tile ends, and
+// a tile's stores drain while the next one multiplies.
+constexpr int WIDE_BUF = 65536, WIDE_SCALES = 2 * WIDE_BUF, WIDE_BIAS = WIDE_SCALES + 512 * SCALE_BLOCKS, WIDE_SLAB = WIDE_BIAS + 2048;
+constexpr int WIDE_LDS = WIDE_SLAB + 4 * 4096;           // two K-tiles, 16 blocks' scale bytes of 512 rows, two tiles' bias, a slab of 32 rows x 128 bytes per wave
+
+template <int FA, bool EXACT>
+__global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p) {
+#ifdef __HIP_DEVICE_COMPILE__
+    typedef typename std::conditional<EXACT, float, bf16>::type T;      // EXACT: fp32 outputs (see the top of the file)
+    extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hi = lane >> 5, l31 = lane & 31, wm = wave >> 1, wn = wave & 1;
+    const int ntiles = p.ntm * p.ntn, nwg = gridDim.x, nk = p.nk;
+    // XCD x's band of tiles, and this workgroup's walk through it
+    const int xcd = (int)blockIdx.x & 7, q8 = ntiles >> 3, r8 = ntiles & 7;
+    const int band = xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8, band_end = band + q8 + (xcd < r8 ? 1 : 0);
+    const int stride = (nwg >> 3) + (xcd < (nwg & 7) ? 1 : 0);
+    int tile = band + ((int)blockIdx.x >> 3);
+    if (tile >= band_end) return;
+    auto place = [&](int id, int& m0, int& n0) {         // bands of four tile rows, column by column (an XCD's 32 CUs: about 4 x 8 tiles)
+        const unsigned d = 4u * (unsigned)p.ntn;
+        unsigned b = __umulhi((unsigned)id, p.band_magic), in = (unsigned)id - b * d;     // floor(2^32 / d): the quotient or one less
+        if (in >= d) { ++b; in -= d; }
+        const unsigned high = min(4u, (unsigned)p.ntm - b * 4u);
+        const unsigned c = high == 4u ? in >> 2 : high == 3u ? __umulhi(in, 0x55555556u) : high == 2u ? in >> 1 : in;
+        m0 = (int)(b * 4u + in - c * high) * 256;
+        n0 = (int)c * 256;
+    };
+    const int64_t K = (int64_t)nk * 128;
+    // ---- fetch stream: 32 pieces of 8 rows x 128 bytes per operand and K-tile, 8 + 8 per wave.  Image: row r at r * 128, its 16-byte chunk c at c ^ ((r >> 1) & 7)
+    unsigned offa[8], offb[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int row = (wave * 8 + i) * 8 + (lane >> 3);
+        const unsigned ch = (unsigned)(((lane & 7) ^ (row >> 1)) & 7) * 16;
+        offa[i] = (unsigned)(row * p.lda) + ch;
+        offb[i] = (unsigned)(row * p.ldb) + ch;
+    }
+    __amdgpu_buffer_rsrc_t ra, rb;
+    int s_tile = tile, s_kt = 0;
+    auto stream_to = [&](int id) {
+        int m = 0, n = 0;
+        if (id < band_end) place(id, m, n);              // (behind the last tile: buffers without a byte -- the two K-tiles fetched ahead touch no memory)
+        ra = rows_rsrc(p.A, m, id < band_end ? min((int64_t)256, p.M - m) : 0, p.lda, K);
+        rb = rows_rsrc(p.B, n, id < band_end ? min((int64_t)256, p.N - n) : 0, p.ldb, K);
+    };
+    auto fetch_a = [&](int i, int buf) { __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, LDS_PTR(lds + buf + (wave * 8 + i) * 1024), 16, offa[i], s_kt * 128, 0, 0); };
+    auto fetch_b = [&](int i, int buf) { __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, LDS_PTR(lds + buf + 32768 + (wave * 8 + i) * 1024), 16, offb[i], s_kt * 128, 0, 0); };
+    auto advance = [&]() {                               // to the stream's next K-tile
+        if (++s_kt == nk) {
+            s_kt = 0;
+            s_tile += stride;
+            stream_to(s_tile);
+        }
+    };
+    // ---- scale words (16 blocks of 512 rows: eight words per thread) and bias, through registers into LDS
+    int sw[8];
+    float bias_reg;
+    auto ask_scales = [&](int id, int kb) {
+        int m, n;
+        place(id, m, n);
+        const int64_t width = (p.nk + 3) & ~3;
+        const __amdgpu_buffer_rsrc_t rsa = rows_rsrc(p.sa, m, min((int64_t)256, p.M - m), p.ldsa, width), rsb = rows_rsrc(p.sb, n, min((int64_t)256, p.N - n), p.ldsb, width);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const unsigned row = k * 64 + (tid >> 2), b = kb + (tid & 3) * 4;
+            sw[k] = __builtin_amdgcn_raw_buffer_load_b32(rsa, row * (unsigned)p.ldsa + b, 0, 0);
+            sw[4 + k] = __builtin_amdgcn_raw_buffer_load_b32(rsb, row * (unsigned)p.ldsb + b, 0, 0);
+        }
+    };
+    auto put_scales = [&]() {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) *reinterpret_cast<int*>(lds + WIDE_SCALES + (k * 64 + (tid >> 2)) * 16 + (tid & 3) * 4) = sw[k];
+    };
+    auto ask_bias = [&](int id) {
+        int m, n;
+        place(id, m, n);
+        bias_reg = p.bias && n + tid < p.N ? p.bias[n + tid] : 0.f;
+    };
+    // ---- fragments
+    const unsigned fra = (unsigned)(wm * 128 + l31) * 128, frb = 32768u + (unsigned)(wn * 128 + l31) * 128;     // + 32 rows = 4 096 bytes each, same exchange
+    const unsigned fx = (unsigned)(l31 >> 1) & 7;
+    auto chunk = [&](unsigned base, int k2, int part) -> i32x4 {           // half a fragment: 16 bytes of a row
+        return *reinterpret_cast<const i32x4*>(lds + base + (((unsigned)(4 * k2 + 2 * hi + part) ^ fx) & 7) * 16);
+    };
+    auto whole = [](const i32x4 (&f)[2]) -> i32x8 { return __builtin_shufflevector(f[0], f[1], 0, 1, 2, 3, 4, 5, 6, 7); };
+    int xa[4], xb[4];
+    auto read_scales = [&](int w) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            xa[i] = *reinterpret_cast<const int*>(lds + WIDE_SCALES + (wm * 128 + i * 32 + l31) * 16 + w * 4);
+            xb[i] = *reinterpret_cast<const int*>(lds + WIDE_SCALES + (256 + wn * 128 + i * 32 + l31) * 16 + w * 4);
+        }
+    };
+    f32x16 acc[4][4];
+    f32x16 zero;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) zero[r] = 0.f;
+    i32x4 fa[2][4][2], fb[2][4][2];                      // [half K-tile][32 rows][16 bytes]
+    // chunk f (0 ... 15) of the fragments of half H in the order the products ask for them: B 0, A 0, A 1, A 2, A 3, B 1, B 2, B 3
+    auto read_chunk = [&](auto hc, int f, unsigned base) __attribute__((always_inline)) {
+        constexpr int H = decltype(hc)::value;
+        const int k = f >> 1, part = f & 1;
+        if (k == 0 || k >= 5) { const int j = k == 0 ? 0 : k - 4; fb[H][j][part] = chunk(base + frb + j * 4096, H, part); }
+        else fa[H][k - 1][part] = chunk(base + fra + (k - 1) * 4096, H, part);
+    };
+    // one half K-tile: the products with the fragments of half P; between them the other half's fragments are read from the buffer at `next`, and with FETCH the stream's
+    // K-tile is fetched into the one at `into`
+    auto half = [&](auto pc, auto firstc, auto fetchc, unsigned next, int into) __attribute__((always_inline)) {
+        constexpr int P = decltype(pc)::value;
+        constexpr bool FIRST = decltype(firstc)::value, FETCH = decltype(fetchc)::value;
+        if constexpr (!EXACT) {
+            // sixteen slots of one matrix instruction (64 cycles), two reads (the first eight) and one fetch
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const int i = k & 3, j = k >> 2;
+                if (k < 8) {
+                    read_chunk(std::integral_constant<int, P ^ 1>{}, 2 * k, next);
+                    read_chunk(std::integral_constant<int, P ^ 1>{}, 2 * k + 1, next);
+                }
+                if constexpr (FETCH) {
+                    if (k & 1) fetch_b(k >> 1, into);
+                    else fetch_a(k >> 1, into);
+                }
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(whole(fb[P][j]), whole(fa[P][i]), FIRST ? zero : acc[i][j], 0, FA, 0, xb[j], 0, xa[i]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        } else {
+            // four groups of sixteen (32 cycles each) with a quarter of the lane's bytes, widened in front of them
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                bf16x8 wa[4], wb[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    wb[k] = widen<0>(fb[P][k][q >> 1][2 * (q & 1)], fb[P][k][q >> 1][2 * (q & 1) + 1], scale_value(xb[k] & 255));
+                    wa[k] = widen<FA>(fa[P][k][q >> 1][2 * (q & 1)], fa[P][k][q >> 1][2 * (q & 1) + 1], scale_value(xa[k] & 255));
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    read_chunk(std::integral_constant<int, P ^ 1>{}, 4 * q + k, next);
+                    if constexpr (FETCH) {
+                        if (k & 1) fetch_b(2 * q + (k >> 1), into);
+                        else fetch_a(2 * q + (k >> 1), into);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        acc[i][k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[k], wa[i], (FIRST && q == 0) ? zero : acc[i][k], 0, 0, 0);
+                }
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {                // (a use in this segment: see blocks_gemm_kernel; the 256 sums fill the accumulation registers)
+                f32x16& s = acc[i][j];
+                asm volatile("" : "+a"(s));
+            }
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    typedef std::integral_constant<int, 0> c0_t;
+    typedef std::integral_constant<int, 1> c1_t;
+    typedef std::integral_constant<bool, false> no_t;
+    typedef std::integral_constant<bool, true> yes_t;
+
+    // ---- prologue
+    ask_scales(tile, 0);
+    ask_bias(tile);
+    put_scales();
+    *reinterpret_cast<float*>(lds + WIDE_BIAS + tid * 4) = bias_reg;
+    stream_to(tile);
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {                        // K-tiles 0 and 1 (the host launches this kernel for K >= 256 only)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { fetch_a(i, b * WIDE_BUF); fetch_b(i, b * WIDE_BUF); }
+        advance();
+    }
+    wait_step<16>();
+    __builtin_amdgcn_s_barrier();
+    unsigned buf = 0;
+#pragma unroll
+    for (int f = 0; f < 16; ++f) read_chunk(c0_t{}, f, buf);
+    int bias_at = WIDE_BIAS, stores = 0;                 // stores: this wave's stores behind the newest fetch, at least
+    while (true) {
+        int m0, n0;
+        place(tile, m0, n0);
+        const int next_tile = tile + stride;
+        const bool last = next_tile >= band_end;
+        read_scales(0);
+        auto ktile = [&](int kt, auto firstc) __attribute__((always_inline)) {
+            half(c0_t{}, firstc, no_t{}, buf, 0);
+            // K-tile kt + 1 has to be complete, and everybody's reads of this buffer (lgkmcnt: ours) done; behind the first K-tile's fetches only the last tile's stores
+            // are younger
+            if (decltype(firstc)::value && stores >= 32) wait_step<32>();
+            else wait_step<0>();
+            __builtin_amdgcn_s_barrier();
+            half(c1_t{}, no_t{}, yes_t{}, buf ^ WIDE_BUF, (int)buf);
+            advance();
+            buf ^= WIDE_BUF;
+            if (((kt + 1) & 15) == 0 && kt + 1 < nk) {   // the next sixteen blocks' bytes (the old ones' last words were read three K-tiles ago)
+                ask_scales(tile, kt + 1);
+                put_scales();
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+            }
+            if (((kt + 1) & 3) == 0) {
+                if (kt + 1 < nk) read_scales(((kt + 1) >> 2) & 3);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    xa[i] = (int)((unsigned)xa[i] >> 8);
+                    xb[i] = (int)((unsigned)xb[i] >> 8);
+                }
+            }
+        };
+        ktile(0, yes_t{});
+        for (int kt = 1; kt < nk; ++kt) ktile(kt, no_t{});
+        if (!last) {
+            ask_scales(next_tile, 0);
+            ask_bias(next_tile);
+        }
+        // ---- epilogue: 32 rows x 128 bytes at a time through the wave's slab (16-byte chunk c of row r at c ^ (r & 7))
+        constexpr int E = 16 / (int)sizeof(T), JU = EXACT ? 1 : 2;              // columns per chunk, fragments per unit
+        uint8_t* const slab = lds + WIDE_SLAB + wave * 4096;
+        int el = lane;                                   // the epilogue's addresses are made here, tile by tile: hoisted out of the tile loop they would fill the registers
+        asm volatile("" : "+v"(el));
+        const int e31 = el & 31, eh = el >> 5;
+        const bool inside = m0 + 256 <= p.M && n0 + 256 <= p.N && !p.accumulate;
+        const int64_t row0 = m0 + wm * 128 + (el >> 3), col0 = n0 + wn * 128 + (el & 7) * E;
+        const int m_left = (int)max((int64_t)-1, min(p.M - row0, (int64_t)256)), n_left = (int)max((int64_t)-1, min(p.N - col0, (int64_t)256));
+        T* out = (T*)p.C + row0 * p.ldc + col0;          // this lane's piece of the slab's rows 0 ... 7
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+#pragma unroll
+            for (int u = 0; u < 4 / JU; ++u) {
+#pragma unroll
+                for (int jj = 0; jj < JU; ++jj)
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int j = u * JU + jj;
+                        const f32x4 b = *reinterpret_cast<const f32x4*>(lds + bias_at + (wn * 128 + j * 32 + g * 8 + eh * 4) * 4);
+                        typedef T vec_t __attribute__((ext_vector_type(4)));
+                        vec_t o;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) o[e] = (T)(acc[i][j][4 * g + e] + b[e]);
+                        const int at = (jj * 32 + g * 8 + eh * 4) * (int)sizeof(T);
+                        *reinterpret_cast<vec_t*>(slab + e31 * 128 + ((((at >> 4) ^ e31) & 7) << 4) + (at & 15)) = o;
+                    }
+                typedef T slab_t __attribute__((ext_vector_type(E)));
+                typedef T out_t __attribute__((ext_vector_type(E), aligned(sizeof(T))));
+                slab_t v[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const slab_t*>(slab + (k * 8 + (el >> 3)) * 128 + (((el ^ (el >> 3)) & 7) << 4));
+                if (inside) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) *reinterpret_cast<out_t*>(out + k * 8 * p.ldc + u * JU * 32) = v[k];
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        if (i * 32 + k * 8 < m_left && u * JU * 32 < n_left) store_out<T, E>(out + k * 8 * p.ldc + u * JU * 32, n_left - u * JU * 32, v[k], EXACT && p.accumulate);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            out += 32 * p.ldc;
+            asm volatile("" : "+v"(out));
+        }
+        if (last) break;
+        stores = inside ? 32 : 0;
+        tile = next_tile;
+        put_scales();                                    // every wave is behind its last read of the old words (a barrier per K-tile)
+        bias_at = bias_at == WIDE_BIAS ? WIDE_BIAS + 1024 : WIDE_BIAS;
+        *reinterpret_cast<float*>(lds + bias_at + tid * 4) = bias_reg;
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
     }
 #endif
 }
@@ -254,23 +574,38 @@ __global__ __launch_bounds__(256) void blocks_fold_kernel(const BlocksArgs p, in
         T __attribute__((ext_vector_type(4))) o;
 #pragma unroll
         for (int e = 0; e < 4; ++e) o[e] = (T)(s[e] + (p.bias && e < left ? p.bias[n + e] : 0.f));
-        store_out<T, 4>((T*)p.C, p.ldc, m, n, left, o, p.accumulate != 0);
+        store_out<T, 4>((T*)p.C + m * p.ldc + n, left, o, p.accumulate != 0);
     }
 }
 
-struct BlocksPlan { int bn, splits, nk_split; };
+struct BlocksPlan { int bm, bn, splits, nk_split; };
 
-// wide tiles where they alone fill the 256 CUs twice; otherwise narrow ones, and a long reduction is split until there are about 512 workgroups, at least eight
-// blocks (16 steps) each
+// 256 x 256 tiles where they fill the 256 CUs; 128 x 256 where those fill them twice; otherwise narrow ones, and a long reduction is split until there are about 512
+// workgroups, at least eight blocks (16 steps) each
 BlocksPlan blocks_plan(int64_t M, int64_t N, int64_t K) {
     const int64_t tm = (M + 127) / 128, nk = K / 128;
-    if (N > 128 && tm * ((N + 255) / 256) >= 512) return {256, 1, (int)nk};
+    if (nk >= 2 && ((M + 255) / 256) * ((N + 255) / 256) >= 256) return {256, 256, 1, (int)nk};
+    if (N > 128 && tm * ((N + 255) / 256) >= 512) return {128, 256, 1, (int)nk};
     const int64_t tiles = tm * ((N + 127) / 128);
     int64_t s = 512 / tiles;
     if (s > nk / 8) s = nk / 8;
-    if (s < 2) return {128, 1, (int)nk};
+    if (s < 2) return {128, 128, 1, (int)nk};
     const int64_t per = ((nk + s - 1) / s + 3) / 4 * 4;
-    return {128, (int)((nk + per - 1) / per), (int)per};
+    return {128, 128, (int)((nk + per - 1) / per), (int)per};
+}
+
+template <int FA>
+int blocks_wide_launch(const BlocksArgs& p, bool out_f32, hipStream_t s) {
+    const int tiles = p.ntm * p.ntn;
+    const dim3 grid(tiles < 256 ? tiles : 256), block(256);
+    if (out_f32) {
+        MERLOT_ENSURE_LDS((blocks_wide_kernel<FA, true>), WIDE_LDS, "merlot_gemm_f8_blocks");
+        hipLaunchKernelGGL((blocks_wide_kernel<FA, true>), grid, block, WIDE_LDS, s, p);
+    } else {
+        MERLOT_ENSURE_LDS((blocks_wide_kernel<FA, false>), WIDE_LDS, "merlot_gemm_f8_blocks");
+        hipLaunchKernelGGL((blocks_wide_kernel<FA, false>), grid, block, WIDE_LDS, s, p);
+    }
+    return MERLOT_OK;
 }
 
 template <int FA, int BN>
@@ -317,12 +652,15 @@ extern "C" int merlot_gemm_f8_blocks(const void* A8, int64_t lda, int fmt_a, con
                  MERLOT_EALIGN, "merlot_gemm_f8_blocks: scale rows must be 4-byte aligned and hold K / 128 bytes");
     const BlocksPlan plan = blocks_plan(M, N, K);
     MERLOT_CHECK(plan.splits == 1 || (workspace && workspace_bytes >= (int64_t)plan.splits * M * N * 4), MERLOT_ESHAPE, "merlot_gemm_f8_blocks: workspace too small");
-    const int64_t ntm = (M + 127) / 128, ntn = (N + plan.bn - 1) / plan.bn;
+    const int64_t ntm = (M + plan.bm - 1) / plan.bm, ntn = (N + plan.bn - 1) / plan.bn;
     MERLOT_CHECK(ntm * ntn < ((int64_t)1 << 31), MERLOT_ESHAPE, "merlot_gemm_f8_blocks: too many tiles");
     const BlocksArgs p = {(const uint8_t*)A8, (const uint8_t*)B8, scale_a, scale_b, lda, ldb, ld_scale_a, ld_scale_b, C, ldc, bias, (float*)workspace, M, N,
-                          (int)(K / 128), plan.nk_split, (int)ntm, (int)ntn, accumulate};
+                          (int)(K / 128), plan.nk_split, (int)ntm, (int)ntn, accumulate, (unsigned)(((uint64_t)1 << 32) / (4 * (uint64_t)ntn))};
     hipStream_t s = (hipStream_t)stream;
-    if (fmt_a == 0) {
+    if (plan.bm == 256) {
+        const int rc = fmt_a == 0 ? blocks_wide_launch<0>(p, out_f32 != 0, s) : blocks_wide_launch<1>(p, out_f32 != 0, s);
+        if (rc != MERLOT_OK) return rc;
+    } else if (fmt_a == 0) {
         if (plan.bn == 256) blocks_launch<0, 256>(p, plan.splits, out_f32 != 0, s);
         else blocks_launch<0, 128>(p, plan.splits, out_f32 != 0, s);
     } else {
