@@ -284,10 +284,10 @@ __global__ __launch_bounds__(256, 2) void blocks_gemm_kernel(const BlocksArgs p)
 constexpr int WIDE_BUF = 65536, WIDE_SCALES = 2 * WIDE_BUF, WIDE_BIAS = WIDE_SCALES + 512 * SCALE_BLOCKS, WIDE_SLAB = WIDE_BIAS + 2048;
 constexpr int WIDE_LDS = WIDE_SLAB + 4 * 4096;           // two K-tiles, 16 blocks' scale bytes of 512 rows, two tiles' bias, a slab of 32 rows x 128 bytes per wave
 
-template <int FA, bool EXACT>
+template <int FA>
 __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p) {
 #ifdef __HIP_DEVICE_COMPILE__
-    typedef typename std::conditional<EXACT, float, bf16>::type T;      // EXACT: fp32 outputs (see the top of the file)
+    typedef bf16 T;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hi = lane >> 5, l31 = lane & 31, wm = wave >> 1, wn = wave & 1;
@@ -390,44 +390,20 @@ __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p)
     auto half = [&](auto pc, auto firstc, auto fetchc, unsigned next, int into) __attribute__((always_inline)) {
         constexpr int P = decltype(pc)::value;
         constexpr bool FIRST = decltype(firstc)::value, FETCH = decltype(fetchc)::value;
-        if constexpr (!EXACT) {
-            // sixteen slots of one matrix instruction (64 cycles), two reads (the first eight) and one fetch
+        // sixteen slots of one matrix instruction (64 cycles), two reads (the first eight) and one fetch
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const int i = k & 3, j = k >> 2;
-                if (k < 8) {
-                    read_chunk(std::integral_constant<int, P ^ 1>{}, 2 * k, next);
-                    read_chunk(std::integral_constant<int, P ^ 1>{}, 2 * k + 1, next);
-                }
-                if constexpr (FETCH) {
-                    if (k & 1) fetch_b(k >> 1, into);
-                    else fetch_a(k >> 1, into);
-                }
-                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(whole(fb[P][j]), whole(fa[P][i]), FIRST ? zero : acc[i][j], 0, FA, 0, xb[j], 0, xa[i]);
-                __builtin_amdgcn_sched_barrier(0);
+        for (int k = 0; k < 16; ++k) {
+            const int i = k & 3, j = k >> 2;
+            if (k < 8) {
+                read_chunk(std::integral_constant<int, P ^ 1>{}, 2 * k, next);
+                read_chunk(std::integral_constant<int, P ^ 1>{}, 2 * k + 1, next);
             }
-        } else {
-            // four groups of sixteen (32 cycles each) with a quarter of the lane's bytes, widened in front of them
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                bf16x8 wa[4], wb[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    wb[k] = widen<0>(fb[P][k][q >> 1][2 * (q & 1)], fb[P][k][q >> 1][2 * (q & 1) + 1], scale_value(xb[k] & 255));
-                    wa[k] = widen<FA>(fa[P][k][q >> 1][2 * (q & 1)], fa[P][k][q >> 1][2 * (q & 1) + 1], scale_value(xa[k] & 255));
-                }
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    read_chunk(std::integral_constant<int, P ^ 1>{}, 4 * q + k, next);
-                    if constexpr (FETCH) {
-                        if (k & 1) fetch_b(2 * q + (k >> 1), into);
-                        else fetch_a(2 * q + (k >> 1), into);
-                    }
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        acc[i][k] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[k], wa[i], (FIRST && q == 0) ? zero : acc[i][k], 0, 0, 0);
-                }
+            if constexpr (FETCH) {
+                if (k & 1) fetch_b(k >> 1, into);
+                else fetch_a(k >> 1, into);
             }
+            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(whole(fb[P][j]), whole(fa[P][i]), FIRST ? zero : acc[i][j], 0, FA, 0, xb[j], 0, xa[i]);
+            __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -499,51 +475,70 @@ __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p)
             ask_scales(next_tile, 0);
             ask_bias(next_tile);
         }
-        // ---- epilogue: 32 rows x 128 bytes at a time through the wave's slab (16-byte chunk c of row r at c ^ (r & 7))
-        constexpr int E = 16 / (int)sizeof(T), JU = EXACT ? 1 : 2;              // columns per chunk, fragments per unit
+        // ---- epilogue: units of 32 rows x 64 columns through the wave's slab (16-byte chunk c of row r at c ^ (r & 7)).  Unit u + 1 is rounded while unit u's writes and reads
+        // travel, and unit u is stored behind that: nothing waits for the slab.
         uint8_t* const slab = lds + WIDE_SLAB + wave * 4096;
         int el = lane;                                   // the epilogue's addresses are made here, tile by tile: hoisted out of the tile loop they would fill the registers
         asm volatile("" : "+v"(el));
         const int e31 = el & 31, eh = el >> 5;
-        const bool inside = m0 + 256 <= p.M && n0 + 256 <= p.N && !p.accumulate;
-        const int64_t row0 = m0 + wm * 128 + (el >> 3), col0 = n0 + wn * 128 + (el & 7) * E;
+        const bool inside = m0 + 256 <= p.M && n0 + 256 <= p.N;
+        const int64_t row0 = m0 + wm * 128 + (el >> 3), col0 = n0 + wn * 128 + (el & 7) * 8;
         const int m_left = (int)max((int64_t)-1, min(p.M - row0, (int64_t)256)), n_left = (int)max((int64_t)-1, min(p.N - col0, (int64_t)256));
-        T* out = (T*)p.C + row0 * p.ldc + col0;          // this lane's piece of the slab's rows 0 ... 7
+        bf16* out = (bf16*)p.C + row0 * p.ldc + col0;    // this lane's piece of the slab's rows 0 ... 7
+        bf16x4 o[8];
+        bf16x8 v[4];
+        f32x4 bias[8];                                   // of the unit's columns: 64 wave columns at a time, two units of columns per 32 rows
+        auto ask = [&](int half) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+            for (int k = 0; k < 8; ++k) bias[k] = *reinterpret_cast<const f32x4*>(lds + bias_at + (wn * 128 + half * 64 + k * 8 + eh * 4) * 4);
+        };
+        auto round = [&](auto uc) __attribute__((always_inline)) {
+            constexpr int U = decltype(uc)::value, I = U & 3, J = (U >> 2) * 2;           // column halves outside: each half's bias is read once
 #pragma unroll
-            for (int u = 0; u < 4 / JU; ++u) {
+            for (int k = 0; k < 8; ++k)
 #pragma unroll
-                for (int jj = 0; jj < JU; ++jj)
+                for (int e = 0; e < 4; ++e) o[k][e] = (bf16)(acc[I][J + (k >> 2)][4 * (k & 3) + e] + bias[k][e]);
+        };
+        auto write = [&]() __attribute__((always_inline)) {
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int j = u * JU + jj;
-                        const f32x4 b = *reinterpret_cast<const f32x4*>(lds + bias_at + (wn * 128 + j * 32 + g * 8 + eh * 4) * 4);
-                        typedef T vec_t __attribute__((ext_vector_type(4)));
-                        vec_t o;
+            for (int k = 0; k < 8; ++k) *reinterpret_cast<bf16x4*>(slab + e31 * 128 + (((k ^ e31) & 7) << 4) + eh * 8) = o[k];
+        };
+        auto read = [&]() __attribute__((always_inline)) {
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) o[e] = (T)(acc[i][j][4 * g + e] + b[e]);
-                        const int at = (jj * 32 + g * 8 + eh * 4) * (int)sizeof(T);
-                        *reinterpret_cast<vec_t*>(slab + e31 * 128 + ((((at >> 4) ^ e31) & 7) << 4) + (at & 15)) = o;
-                    }
-                typedef T slab_t __attribute__((ext_vector_type(E)));
-                typedef T out_t __attribute__((ext_vector_type(E), aligned(sizeof(T))));
-                slab_t v[4];
+            for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const bf16x8*>(slab + (k * 8 + (el >> 3)) * 128 + (((el ^ (el >> 3)) & 7) << 4));
+        };
+        auto store = [&](auto uc) __attribute__((always_inline)) {
+            constexpr int U = decltype(uc)::value, I = U & 3, C0 = (U >> 2) * 64;
+            typedef bf16 out_t __attribute__((ext_vector_type(8), aligned(2)));
+            if (inside) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const slab_t*>(slab + (k * 8 + (el >> 3)) * 128 + (((el ^ (el >> 3)) & 7) << 4));
-                if (inside) {
+                for (int k = 0; k < 4; ++k) *reinterpret_cast<out_t*>(out + (I * 32 + k * 8) * p.ldc + C0) = v[k];
+            } else {
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) *reinterpret_cast<out_t*>(out + k * 8 * p.ldc + u * JU * 32) = v[k];
-                } else {
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        if (i * 32 + k * 8 < m_left && u * JU * 32 < n_left) store_out<T, E>(out + k * 8 * p.ldc + u * JU * 32, n_left - u * JU * 32, v[k], EXACT && p.accumulate);
-                }
-                __builtin_amdgcn_sched_barrier(0);
+                for (int k = 0; k < 4; ++k)
+                    if (I * 32 + k * 8 < m_left && C0 < n_left) store_out<bf16, 8>(out + (I * 32 + k * 8) * p.ldc + C0, n_left - C0, v[k], false);
             }
-            out += 32 * p.ldc;
-            asm volatile("" : "+v"(out));
-        }
+        };
+        auto unit = [&](auto uc) __attribute__((always_inline)) {
+            constexpr int U = decltype(uc)::value;
+            if constexpr (U == 4) ask(1);
+            round(uc);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (U > 0) store(std::integral_constant<int, U - 1>{});
+            write();
+            __builtin_amdgcn_sched_barrier(0);
+            read();                                      // (LDS operations of a wave keep their order)
+        };
+        ask(0);
+        unit(std::integral_constant<int, 0>{});
+        unit(std::integral_constant<int, 1>{});
+        unit(std::integral_constant<int, 2>{});
+        unit(std::integral_constant<int, 3>{});
+        unit(std::integral_constant<int, 4>{});
+        unit(std::integral_constant<int, 5>{});
+        unit(std::integral_constant<int, 6>{});
+        unit(std::integral_constant<int, 7>{});
+        store(std::integral_constant<int, 7>{});
         if (last) break;
         stores = inside ? 32 : 0;
         tile = next_tile;
@@ -580,11 +575,12 @@ __global__ __launch_bounds__(256) void blocks_fold_kernel(const BlocksArgs p, in
 
 struct BlocksPlan { int bm, bn, splits, nk_split; };
 
-// 256 x 256 tiles where they fill the 256 CUs; 128 x 256 where those fill them twice; otherwise narrow ones, and a long reduction is split until there are about 512
-// workgroups, at least eight blocks (16 steps) each
-BlocksPlan blocks_plan(int64_t M, int64_t N, int64_t K) {
+// bf16 outputs of long enough reductions take 256 x 256 tiles where they fill the 256 CUs: 8192^3 396 us against 527 with 128 x 256, 32768 x 1024 x 4096 110 : 138,
+// 32768 x 4096 x 1024 160 : 170; at K = 768 (101376 x 2304) 265 : 258, and fp32 outputs gain nothing there (the bf16 matrix instructions are the bound either way).  128 x 256 where
+// those fill the CUs twice; otherwise narrow tiles, and a long reduction is split until there are about 512 workgroups, at least eight blocks (16 steps) each
+BlocksPlan blocks_plan(int64_t M, int64_t N, int64_t K, bool out_f32) {
     const int64_t tm = (M + 127) / 128, nk = K / 128;
-    if (nk >= 2 && ((M + 255) / 256) * ((N + 255) / 256) >= 256) return {256, 256, 1, (int)nk};
+    if (!out_f32 && nk >= 8 && ((M + 255) / 256) * ((N + 255) / 256) >= 256) return {256, 256, 1, (int)nk};
     if (N > 128 && tm * ((N + 255) / 256) >= 512) return {128, 256, 1, (int)nk};
     const int64_t tiles = tm * ((N + 127) / 128);
     int64_t s = 512 / tiles;
@@ -595,16 +591,10 @@ BlocksPlan blocks_plan(int64_t M, int64_t N, int64_t K) {
 }
 
 template <int FA>
-int blocks_wide_launch(const BlocksArgs& p, bool out_f32, hipStream_t s) {
+int blocks_wide_launch(const BlocksArgs& p, hipStream_t s) {
     const int tiles = p.ntm * p.ntn;
-    const dim3 grid(tiles < 256 ? tiles : 256), block(256);
-    if (out_f32) {
-        MERLOT_ENSURE_LDS((blocks_wide_kernel<FA, true>), WIDE_LDS, "merlot_gemm_f8_blocks");
-        hipLaunchKernelGGL((blocks_wide_kernel<FA, true>), grid, block, WIDE_LDS, s, p);
-    } else {
-        MERLOT_ENSURE_LDS((blocks_wide_kernel<FA, false>), WIDE_LDS, "merlot_gemm_f8_blocks");
-        hipLaunchKernelGGL((blocks_wide_kernel<FA, false>), grid, block, WIDE_LDS, s, p);
-    }
+    MERLOT_ENSURE_LDS((blocks_wide_kernel<FA>), WIDE_LDS, "merlot_gemm_f8_blocks");
+    hipLaunchKernelGGL((blocks_wide_kernel<FA>), dim3(tiles < 256 ? tiles : 256), dim3(256), WIDE_LDS, s, p);
     return MERLOT_OK;
 }
 
@@ -634,7 +624,7 @@ void blocks_launch(const BlocksArgs& p, int splits, bool out_f32, hipStream_t s)
 
 extern "C" int64_t merlot_gemm_f8_blocks_workspace_bytes(int64_t M, int64_t N, int64_t K) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    const BlocksPlan plan = blocks_plan(M, N, K);
+    const BlocksPlan plan = blocks_plan(M, N, K, true);      // (bf16 outputs never split further than fp32 ones)
     return plan.splits > 1 ? (int64_t)plan.splits * M * N * 4 : 0;
 }
 
@@ -650,7 +640,7 @@ extern "C" int merlot_gemm_f8_blocks(const void* A8, int64_t lda, int fmt_a, con
     MERLOT_CHECK(ld_scale_a >= K / 128 && ld_scale_b >= K / 128 && ld_scale_a % 4 == 0 && ld_scale_b % 4 == 0 && ld_scale_a < (1 << 22) && ld_scale_b < (1 << 22) &&
                      (((uintptr_t)scale_a | (uintptr_t)scale_b) & 3) == 0,
                  MERLOT_EALIGN, "merlot_gemm_f8_blocks: scale rows must be 4-byte aligned and hold K / 128 bytes");
-    const BlocksPlan plan = blocks_plan(M, N, K);
+    const BlocksPlan plan = blocks_plan(M, N, K, out_f32 != 0);
     MERLOT_CHECK(plan.splits == 1 || (workspace && workspace_bytes >= (int64_t)plan.splits * M * N * 4), MERLOT_ESHAPE, "merlot_gemm_f8_blocks: workspace too small");
     const int64_t ntm = (M + plan.bm - 1) / plan.bm, ntn = (N + plan.bn - 1) / plan.bn;
     MERLOT_CHECK(ntm * ntn < ((int64_t)1 << 31), MERLOT_ESHAPE, "merlot_gemm_f8_blocks: too many tiles");
@@ -658,7 +648,7 @@ extern "C" int merlot_gemm_f8_blocks(const void* A8, int64_t lda, int fmt_a, con
                           (int)(K / 128), plan.nk_split, (int)ntm, (int)ntn, accumulate, (unsigned)(((uint64_t)1 << 32) / (4 * (uint64_t)ntn))};
     hipStream_t s = (hipStream_t)stream;
     if (plan.bm == 256) {
-        const int rc = fmt_a == 0 ? blocks_wide_launch<0>(p, out_f32 != 0, s) : blocks_wide_launch<1>(p, out_f32 != 0, s);
+        const int rc = fmt_a == 0 ? blocks_wide_launch<0>(p, s) : blocks_wide_launch<1>(p, s);
         if (rc != MERLOT_OK) return rc;
     } else if (fmt_a == 0) {
         if (plan.bn == 256) blocks_launch<0, 256>(p, plan.splits, out_f32 != 0, s);
