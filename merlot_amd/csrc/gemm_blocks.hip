@@ -31,14 +31,15 @@ __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint8_t* p, in
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(p + row0 * ld), 0, rows > 0 ? (int)((rows - 1) * ld + width) : 0, 0x00020000);
 }
 
-// up to E consecutive columns at c, `left` of which exist; add: onto what is there (fp32 only)
+// up to E consecutive columns at c, `left` of which exist; add: onto what is there (fp32 only).  Outputs are stored past the caches (non-temporal): kept in the L2, a
+// large output drives out the operands that the neighbouring tiles are about to read -- 101376 x 2304 x 768 takes 262 us that way and 194 us this way.
 template <typename T, int E>
 __device__ __forceinline__ void store_out(T* c, int64_t left, T __attribute__((ext_vector_type(E))) v, bool add) {
     typedef T vec_t __attribute__((ext_vector_type(E), aligned(sizeof(T))));
     if (left >= E) {
         if constexpr (sizeof(T) == 4)
             if (add) v += *reinterpret_cast<const vec_t*>(c);
-        *reinterpret_cast<vec_t*>(c) = v;
+        __builtin_nontemporal_store((vec_t)v, reinterpret_cast<vec_t*>(c));
     } else {
 #pragma unroll
         for (int e = 0; e < E; ++e)
@@ -284,7 +285,8 @@ __global__ __launch_bounds__(256, 2) void blocks_gemm_kernel(const BlocksArgs p)
 constexpr int WIDE_BUF = 65536, WIDE_SCALES = 2 * WIDE_BUF, WIDE_BIAS = WIDE_SCALES + 512 * SCALE_BLOCKS, WIDE_SLAB = WIDE_BIAS + 2048;
 constexpr int WIDE_LDS = WIDE_SLAB + 4 * 4096;           // two K-tiles, 16 blocks' scale bytes of 512 rows, two tiles' bias, a slab of 32 rows x 128 bytes per wave
 
-template <int FA>
+// LINES: rows of C start at multiples of 64 bytes -- stored past the caches (a template: two branches with the same store would be merged into an ordinary one)
+template <int FA, bool LINES>
 __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p) {
 #ifdef __HIP_DEVICE_COMPILE__
     typedef bf16 T;
@@ -512,7 +514,11 @@ __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p)
             typedef bf16 out_t __attribute__((ext_vector_type(8), aligned(2)));
             if (inside) {
 #pragma unroll
-                for (int k = 0; k < 4; ++k) *reinterpret_cast<out_t*>(out + (I * 32 + k * 8) * p.ldc + C0) = v[k];
+                for (int k = 0; k < 4; ++k) {
+                    out_t* c = reinterpret_cast<out_t*>(out + (I * 32 + k * 8) * p.ldc + C0);
+                    if constexpr (LINES) __builtin_nontemporal_store((out_t)v[k], c);
+                    else *c = v[k];
+                }
             } else {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
@@ -575,12 +581,14 @@ __global__ __launch_bounds__(256) void blocks_fold_kernel(const BlocksArgs p, in
 
 struct BlocksPlan { int bm, bn, splits, nk_split; };
 
-// bf16 outputs of long enough reductions take 256 x 256 tiles where they fill the 256 CUs: 8192^3 396 us against 527 with 128 x 256, 32768 x 1024 x 4096 110 : 138,
-// 32768 x 4096 x 1024 160 : 170; at K = 768 (101376 x 2304) 265 : 258, and fp32 outputs gain nothing there (the bf16 matrix instructions are the bound either way).  128 x 256 where
-// those fill the CUs twice; otherwise narrow tiles, and a long reduction is split until there are about 512 workgroups, at least eight blocks (16 steps) each
-BlocksPlan blocks_plan(int64_t M, int64_t N, int64_t K, bool out_f32) {
+// bf16 outputs take 256 x 256 tiles where those fill the 256 CUs and the reduction is long enough to pay for an epilogue nobody covers (us, 128 x 256 tiles : 256 x 256):
+//   101376 x 2304 x 384 139 : 138, x 512 161 : 139, x 768 224 : 200; 65536 x 768 x 768 55 : 49; 32768 x 4096 x 1024 159 : 142; 8192^3 513 : 400
+// With rows of C that start inside a 64-byte sector their 128-byte row pieces are written as parts of lines, past the caches or not: 101376 x 2296 x 768 225 : 306, and only a
+// long reduction hides it (30000 x 2296 x 2048 163 : 147, x 4096 297 : 254; 4099 x 50370 x 2048 467 : 476).  fp32 outputs gain nothing (the bf16 matrix instructions are the bound either way).
+// 128 x 256 where those fill the CUs twice; otherwise narrow tiles, and a long reduction is split until there are about 512 workgroups, at least eight blocks (16 steps) each
+BlocksPlan blocks_plan(int64_t M, int64_t N, int64_t K, bool out_bf16, bool whole_lines) {
     const int64_t tm = (M + 127) / 128, nk = K / 128;
-    if (!out_f32 && nk >= 8 && ((M + 255) / 256) * ((N + 255) / 256) >= 256) return {256, 256, 1, (int)nk};
+    if (out_bf16 && nk >= (whole_lines ? 4 : 16) && ((M + 255) / 256) * ((N + 255) / 256) >= 256) return {256, 256, 1, (int)nk};
     if (N > 128 && tm * ((N + 255) / 256) >= 512) return {128, 256, 1, (int)nk};
     const int64_t tiles = tm * ((N + 127) / 128);
     int64_t s = 512 / tiles;
@@ -590,11 +598,11 @@ BlocksPlan blocks_plan(int64_t M, int64_t N, int64_t K, bool out_f32) {
     return {128, 128, (int)((nk + per - 1) / per), (int)per};
 }
 
-template <int FA>
+template <int FA, bool LINES>
 int blocks_wide_launch(const BlocksArgs& p, hipStream_t s) {
     const int tiles = p.ntm * p.ntn;
-    MERLOT_ENSURE_LDS((blocks_wide_kernel<FA>), WIDE_LDS, "merlot_gemm_f8_blocks");
-    hipLaunchKernelGGL((blocks_wide_kernel<FA>), dim3(tiles < 256 ? tiles : 256), dim3(256), WIDE_LDS, s, p);
+    MERLOT_ENSURE_LDS((blocks_wide_kernel<FA, LINES>), WIDE_LDS, "merlot_gemm_f8_blocks");
+    hipLaunchKernelGGL((blocks_wide_kernel<FA, LINES>), dim3(tiles < 256 ? tiles : 256), dim3(256), WIDE_LDS, s, p);
     return MERLOT_OK;
 }
 
@@ -624,7 +632,7 @@ void blocks_launch(const BlocksArgs& p, int splits, bool out_f32, hipStream_t s)
 
 extern "C" int64_t merlot_gemm_f8_blocks_workspace_bytes(int64_t M, int64_t N, int64_t K) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    const BlocksPlan plan = blocks_plan(M, N, K, true);      // (bf16 outputs never split further than fp32 ones)
+    const BlocksPlan plan = blocks_plan(M, N, K, false, false);      // (wide tiles split nothing)
     return plan.splits > 1 ? (int64_t)plan.splits * M * N * 4 : 0;
 }
 
@@ -640,7 +648,8 @@ extern "C" int merlot_gemm_f8_blocks(const void* A8, int64_t lda, int fmt_a, con
     MERLOT_CHECK(ld_scale_a >= K / 128 && ld_scale_b >= K / 128 && ld_scale_a % 4 == 0 && ld_scale_b % 4 == 0 && ld_scale_a < (1 << 22) && ld_scale_b < (1 << 22) &&
                      (((uintptr_t)scale_a | (uintptr_t)scale_b) & 3) == 0,
                  MERLOT_EALIGN, "merlot_gemm_f8_blocks: scale rows must be 4-byte aligned and hold K / 128 bytes");
-    const BlocksPlan plan = blocks_plan(M, N, K, out_f32 != 0);
+    const bool whole_lines = (((uintptr_t)C | (uint64_t)ldc * (out_f32 ? 4 : 2)) & 63) == 0;
+    const BlocksPlan plan = blocks_plan(M, N, K, !out_f32, whole_lines);
     MERLOT_CHECK(plan.splits == 1 || (workspace && workspace_bytes >= (int64_t)plan.splits * M * N * 4), MERLOT_ESHAPE, "merlot_gemm_f8_blocks: workspace too small");
     const int64_t ntm = (M + plan.bm - 1) / plan.bm, ntn = (N + plan.bn - 1) / plan.bn;
     MERLOT_CHECK(ntm * ntn < ((int64_t)1 << 31), MERLOT_ESHAPE, "merlot_gemm_f8_blocks: too many tiles");
@@ -648,7 +657,8 @@ extern "C" int merlot_gemm_f8_blocks(const void* A8, int64_t lda, int fmt_a, con
                           (int)(K / 128), plan.nk_split, (int)ntm, (int)ntn, accumulate, (unsigned)(((uint64_t)1 << 32) / (4 * (uint64_t)ntn))};
     hipStream_t s = (hipStream_t)stream;
     if (plan.bm == 256) {
-        const int rc = fmt_a == 0 ? blocks_wide_launch<0>(p, s) : blocks_wide_launch<1>(p, s);
+        const int rc = fmt_a == 0 ? (whole_lines ? blocks_wide_launch<0, true>(p, s) : blocks_wide_launch<0, false>(p, s))
+                                  : (whole_lines ? blocks_wide_launch<1, true>(p, s) : blocks_wide_launch<1, false>(p, s));
         if (rc != MERLOT_OK) return rc;
     } else if (fmt_a == 0) {
         if (plan.bn == 256) blocks_launch<0, 256>(p, plan.splits, out_f32 != 0, s);
