@@ -2,35 +2,35 @@
 //
 //   N = sqrt(sum over tensors and elements of g^2)      out = g * (clip / max(N, clip))
 //
-// Two passes over the gradients (no element can be scaled before the last one is summed), both bound by memory, in two launches per 128 tensors: the tensors'
-// addresses and sizes travel as kernel arguments -- no table in device memory, nothing to copy, nothing kept from one call for the next, and a captured call
-// replays as it is.  Squares are summed in 64 bits (a model's 2 * 10^8 addends; half the fp32 rate is far above what memory delivers) in a fixed order: each
-// workgroup leaves one partial, every workgroup of the second pass adds all partials up by itself (at most 16 KiB per 128 tensors, from the L2), which saves the
-// launch between the passes.  The second pass walks the chunks backwards: what the first pass read last is still in the memory-side cache.
+// Two passes over the gradients (no element can be scaled before the last one is summed), both bound by memory, in two launches: the tensors' addresses and sizes travel
+// as kernel arguments, those of more than 112 tensors by way of small launches that write them into a table in the workspace -- nothing to copy, nothing kept from one call
+// for the next, and a captured call replays as it is.  Squares are summed in 64 bits (a model's 2 * 10^8 addends; half the fp32 rate is far above what memory
+// delivers) in a fixed order: each workgroup leaves one partial, every workgroup of the second pass adds all partials up by itself (8 KiB from the L2), which
+// saves the launch between the passes.
 #include <stdlib.h>
 #include <algorithm>
 #include "common.h"
 
 namespace {
 
-constexpr int CLIP_TENSORS = 128;                        // tensors per launch: 128 x (address, address, size, first chunk) = 3.6 KiB of arguments
-constexpr int CLIP_GROUPS = 2048;                        // 16-byte groups of the input per chunk (32 KiB)
-constexpr int CLIP_BLOCKS = 2048;                        // workgroups (= partials) per launch at most
+constexpr int CLIP_TENSORS = 112;                        // tensors whose entries fit a launch's arguments: 3.5 KiB
+constexpr int CLIP_CHUNK = 4096;                         // elements per chunk, whatever their type: stretches of chunks are equal work
+constexpr int CLIP_BLOCKS = 1536;                        // workgroups (= partials) at most
 
-struct ClipTable {
-    const void* in[CLIP_TENSORS];
-    void* out[CLIP_TENSORS];
-    int64_t n[CLIP_TENSORS];
-    uint32_t chunk0[CLIP_TENSORS + 1];                   // first chunk of each tensor; [count] = all chunks
-    uint32_t in16[CLIP_TENSORS / 32], out16[CLIP_TENSORS / 32];   // bit: the tensor is bf16
-    int count;
+struct ClipEntry {
+    const void* in;
+    void* out;
+    int64_t n;
+    uint32_t chunk0;                                     // the tensor's first chunk
+    uint32_t types;                                      // bit 0: in is bf16, bit 1: out is bf16
 };
+struct ClipTable { ClipEntry e[CLIP_TENSORS]; };
 
-__device__ __forceinline__ int clip_find(const ClipTable& t, uint32_t chunk) {   // the tensor a chunk belongs to
-    int lo = 0, hi = t.count;
+__device__ __forceinline__ int clip_find(const ClipEntry* t, int count, uint32_t chunk) {   // the tensor a chunk belongs to
+    int lo = 0, hi = count;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (t.chunk0[mid] <= chunk) lo = mid;
+        if (t[mid].chunk0 <= chunk) lo = mid;
         else hi = mid;
     }
     return lo;
@@ -39,10 +39,12 @@ __device__ __forceinline__ int clip_find(const ClipTable& t, uint32_t chunk) {  
 template <typename T> struct Group16 { typedef T type __attribute__((ext_vector_type(16 / sizeof(T)))); };
 
 // elements i0 ... i0 + E - 1 of g as one aligned 16-byte load, those outside [0, n) as zeros
-template <typename T, int E = 16 / sizeof(T)>
+template <typename T, bool LAST, int E = 16 / sizeof(T)>
 __device__ __forceinline__ void clip_load(const T* g, int64_t i0, int64_t n, float (&v)[E]) {
     if (i0 >= 0 && i0 + E <= n) {
-        const typename Group16<T>::type t = *reinterpret_cast<const typename Group16<T>::type*>(g + i0);
+        typename Group16<T>::type t;                     // LAST: nobody reads it again -- past the caches (one buffer of 223 M values 479 -> 471 us)
+        if constexpr (LAST) t = __builtin_nontemporal_load(reinterpret_cast<const typename Group16<T>::type*>(g + i0));
+        else t = *reinterpret_cast<const typename Group16<T>::type*>(g + i0);
 #pragma unroll
         for (int e = 0; e < E; ++e) v[e] = (float)t[e];
     } else {
@@ -57,20 +59,17 @@ __device__ __forceinline__ int clip_shift(const void* g) { return (int)(((uintpt
 
 template <typename T>
 __device__ __forceinline__ double clip_square_sum(const T* g, int64_t n, uint32_t chunk) {
-    constexpr int E = 16 / sizeof(T), U = 4;
+    constexpr int E = 16 / sizeof(T), U = CLIP_CHUNK / E / 256;
     const int shift = clip_shift<T>(g);
-    const int64_t first = (int64_t)chunk * CLIP_GROUPS;
+    const int64_t first = (int64_t)chunk * (CLIP_CHUNK / E);
     double s = 0.0;
+    float v[U][E];
 #pragma unroll
-    for (int k = 0; k < CLIP_GROUPS / 256; k += U) {
-        float v[U][E];
+    for (int u = 0; u < U; ++u) clip_load<T, false>(g, (first + u * 256 + threadIdx.x) * E - shift, n, v[u]);
 #pragma unroll
-        for (int u = 0; u < U; ++u) clip_load<T>(g, (first + (k + u) * 256 + threadIdx.x) * E - shift, n, v[u]);
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int e = 0; e < E; ++e) s += (double)v[u][e] * (double)v[u][e];
-    }
+        for (int e = 0; e < E; ++e) s += (double)v[u][e] * (double)v[u][e];
     return s;
 }
 
@@ -84,67 +83,90 @@ __device__ __forceinline__ double block_sum_f64(double s) {
     return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
-__global__ __launch_bounds__(256) void clip_norm_kernel(const ClipTable t, double* __restrict__ part) {
+// a workgroup's chunks: a contiguous stretch, so that it looks its tensor up once and walks on from there
+__device__ __forceinline__ void clip_norm(const ClipEntry* t, int count, uint32_t chunks, double* part) {
+    uint32_t c = (uint32_t)((uint64_t)chunks * blockIdx.x / gridDim.x);
+    const uint32_t end = (uint32_t)((uint64_t)chunks * (blockIdx.x + 1) / gridDim.x);
     double s = 0.0;
-    for (uint32_t c = blockIdx.x; c < t.chunk0[t.count]; c += gridDim.x) {
-        const int i = clip_find(t, c);
-        if (t.in16[i >> 5] >> (i & 31) & 1) s += clip_square_sum<bf16>((const bf16*)t.in[i], t.n[i], c - t.chunk0[i]);
-        else s += clip_square_sum<float>((const float*)t.in[i], t.n[i], c - t.chunk0[i]);
+    int i = c < end ? clip_find(t, count, c) : 0;
+    for (; c < end; ++c) {
+        while (i + 1 < count && t[i + 1].chunk0 <= c) ++i;
+        const ClipEntry e = t[i];
+        if (e.types & 1) s += clip_square_sum<bf16>((const bf16*)e.in, e.n, c - e.chunk0);
+        else s += clip_square_sum<float>((const float*)e.in, e.n, c - e.chunk0);
     }
     s = block_sum_f64(s);
     if (threadIdx.x == 0) part[blockIdx.x] = s;
 }
+__global__ __launch_bounds__(256) void clip_norm_kernel(const ClipTable t, int count, uint32_t chunks, double* __restrict__ part) { clip_norm(t.e, count, chunks, part); }
+__global__ __launch_bounds__(256) void clip_norm_table_kernel(const ClipEntry* __restrict__ t, int count, uint32_t chunks, double* __restrict__ part) {
+    clip_norm(t, count, chunks, part);
+}
+// up to CLIP_TENSORS entries from the arguments into a table in the workspace
+__global__ __launch_bounds__(128) void clip_table_kernel(const ClipTable t, ClipEntry* __restrict__ out, int count) {
+    if ((int)threadIdx.x < count) out[threadIdx.x] = t.e[threadIdx.x];
+}
 
 template <typename TI, typename TO>
 __device__ __forceinline__ void clip_scale(const TI* g, TO* out, int64_t n, uint32_t chunk, float coef) {
-    constexpr int E = 16 / sizeof(TI), U = 4;
+    constexpr int E = 16 / sizeof(TI), U = CLIP_CHUNK / E / 256;
     const int shift = clip_shift<TI>(g);
     const bool wide = ((uintptr_t)(out - shift) & 15) == 0;      // the output's groups are aligned where the input's are
-    const int64_t first = (int64_t)chunk * CLIP_GROUPS;
+    const int64_t first = (int64_t)chunk * (CLIP_CHUNK / E);
+    float v[U][E];
 #pragma unroll
-    for (int k = 0; k < CLIP_GROUPS / 256; k += U) {
-        float v[U][E];
+    for (int u = 0; u < U; ++u) clip_load<TI, true>(g, (first + u * 256 + threadIdx.x) * E - shift, n, v[u]);
 #pragma unroll
-        for (int u = 0; u < U; ++u) clip_load<TI>(g, (first + (k + u) * 256 + threadIdx.x) * E - shift, n, v[u]);
+    for (int u = 0; u < U; ++u) {
+        const int64_t i0 = (first + u * 256 + threadIdx.x) * E - shift;
+        if (wide && i0 >= 0 && i0 + E <= n) {
+            typedef TO vec_t __attribute__((ext_vector_type(E), aligned(8)));
+            vec_t o;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int64_t i0 = (first + (k + u) * 256 + threadIdx.x) * E - shift;
-            if (wide && i0 >= 0 && i0 + E <= n) {
-                typedef TO vec_t __attribute__((ext_vector_type(E), aligned(8)));
-                vec_t o;
+            for (int e = 0; e < E; ++e) o[e] = (TO)(v[u][e] * coef);
+            // past the caches too, so that the inputs the first pass read last stay there (533 -> 495 us); a lane's two pieces of a wider type are no whole lines
+            if constexpr (sizeof(TO) <= sizeof(TI)) __builtin_nontemporal_store(o, reinterpret_cast<vec_t*>(out + i0));
+            else *reinterpret_cast<vec_t*>(out + i0) = o;
+        } else {
 #pragma unroll
-                for (int e = 0; e < E; ++e) o[e] = (TO)(v[u][e] * coef);
-                *reinterpret_cast<vec_t*>(out + i0) = o;
-            } else {
-#pragma unroll
-                for (int e = 0; e < E; ++e)
-                    if (i0 + e >= 0 && i0 + e < n) out[i0 + e] = (TO)(v[u][e] * coef);
-            }
+            for (int e = 0; e < E; ++e)
+                if (i0 + e >= 0 && i0 + e < n) out[i0 + e] = (TO)(v[u][e] * coef);
         }
     }
 }
 
-// norm (written by the first workgroup of the first launch) and, with clip > 0, the scaled tensors
-__global__ __launch_bounds__(256) void clip_scale_kernel(const ClipTable t, const double* __restrict__ part, int nparts, float clip, float* __restrict__ norm) {
+// norm (written by the first workgroup) and, with clip > 0, the scaled tensors
+__device__ __forceinline__ void clip_scale_all(const ClipEntry* t, int count, uint32_t chunks, const double* part, int nparts, float clip, float* norm) {
     double s = 0.0;
     for (int i = threadIdx.x; i < nparts; i += 256) s += part[i];
     s = block_sum_f64(s);
     const float total = (float)sqrt(s);
-    if (norm && blockIdx.x == 0 && threadIdx.x == 0) norm[0] = total;
+    if (blockIdx.x == 0 && threadIdx.x == 0) norm[0] = total;
     if (!(clip > 0.f)) return;
     const float coef = clip / (total < clip ? clip : total);     // a NaN norm stays NaN
-    const uint32_t chunks = t.chunk0[t.count];
-    for (uint32_t k = blockIdx.x; k < chunks; k += gridDim.x) {
-        const uint32_t c = chunks - 1 - k;
-        const int i = clip_find(t, c);
-        const bool in16 = t.in16[i >> 5] >> (i & 31) & 1, out16 = t.out16[i >> 5] >> (i & 31) & 1;
-        if (coef == 1.f && t.in[i] == t.out[i]) continue;        // in place and nothing to clip: every element stays as it is
-        const uint32_t lc = c - t.chunk0[i];
-        if (in16 && out16) clip_scale<bf16, bf16>((const bf16*)t.in[i], (bf16*)t.out[i], t.n[i], lc, coef);
-        else if (in16) clip_scale<bf16, float>((const bf16*)t.in[i], (float*)t.out[i], t.n[i], lc, coef);
-        else if (out16) clip_scale<float, bf16>((const float*)t.in[i], (bf16*)t.out[i], t.n[i], lc, coef);
-        else clip_scale<float, float>((const float*)t.in[i], (float*)t.out[i], t.n[i], lc, coef);
+    // the last stretch first: what the first pass read last is still in the memory-side cache
+    const uint32_t b = gridDim.x - 1 - blockIdx.x, first = (uint32_t)((uint64_t)chunks * b / gridDim.x);
+    uint32_t c = (uint32_t)((uint64_t)chunks * (b + 1) / gridDim.x);
+    int i = c > first ? clip_find(t, count, c - 1) : 0;
+    while (c > first) {
+        --c;
+        while (t[i].chunk0 > c) --i;
+        const ClipEntry e = t[i];
+        if (coef == 1.f && e.in == e.out) continue;              // in place and nothing to clip: every element stays as it is
+        const uint32_t lc = c - e.chunk0;
+        if (e.types == 3) clip_scale<bf16, bf16>((const bf16*)e.in, (bf16*)e.out, e.n, lc, coef);
+        else if (e.types == 1) clip_scale<bf16, float>((const bf16*)e.in, (float*)e.out, e.n, lc, coef);
+        else if (e.types == 2) clip_scale<float, bf16>((const float*)e.in, (bf16*)e.out, e.n, lc, coef);
+        else clip_scale<float, float>((const float*)e.in, (float*)e.out, e.n, lc, coef);
     }
+}
+__global__ __launch_bounds__(256) void clip_scale_kernel(const ClipTable t, int count, uint32_t chunks, const double* __restrict__ part, int nparts, float clip,
+                                                         float* __restrict__ norm) {
+    clip_scale_all(t.e, count, chunks, part, nparts, clip, norm);
+}
+__global__ __launch_bounds__(256) void clip_scale_table_kernel(const ClipEntry* __restrict__ t, int count, uint32_t chunks, const double* __restrict__ part, int nparts,
+                                                               float clip, float* __restrict__ norm) {
+    clip_scale_all(t, count, chunks, part, nparts, clip, norm);
 }
 
 struct Span { uint64_t lo, hi; };
@@ -152,7 +174,7 @@ struct Span { uint64_t lo, hi; };
 }  // namespace
 
 extern "C" int64_t merlot_clip_workspace_bytes(int64_t n) {
-    return n <= 0 ? 0 : (n + CLIP_TENSORS - 1) / CLIP_TENSORS * CLIP_BLOCKS * 8;
+    return n <= 0 ? 0 : CLIP_BLOCKS * 8 + (n > CLIP_TENSORS ? n * (int64_t)sizeof(ClipEntry) : 0);
 }
 
 extern "C" int merlot_clip_by_global_norm(const int64_t* in, const int64_t* out, const int64_t* numel, const uint8_t* types, int64_t n, float clip, float* norm,
@@ -200,38 +222,32 @@ extern "C" int merlot_clip_by_global_norm(const int64_t* in, const int64_t* out,
     }
     hipStream_t s = (hipStream_t)stream;
     double* part = (double*)workspace;
-    const int64_t launches = (n + CLIP_TENSORS - 1) / CLIP_TENSORS;
-    int nparts = 0;
-    for (int pass = 0; pass < 2; ++pass) {
-        for (int64_t l = 0; l < launches; ++l) {
-            ClipTable t;
-            t.count = 0;
-            uint64_t chunks = 0;
-            for (int k = 0; k < CLIP_TENSORS / 32; ++k) t.in16[k] = t.out16[k] = 0;
-            for (int64_t i = l * CLIP_TENSORS; i < n && i < (l + 1) * CLIP_TENSORS; ++i) {
-                if (numel[i] == 0) continue;
-                const int k = t.count++;
-                const int es = types[i] & 1 ? 2 : 4;
-                const uint64_t groups = ((uint64_t)numel[i] * es + ((uint64_t)in[i] & 15) + 15) / 16;
-                t.in[k] = (const void*)in[i];
-                t.out[k] = clip > 0.f ? (void*)out[i] : nullptr;
-                t.n[k] = numel[i];
-                t.chunk0[k] = (uint32_t)chunks;
-                t.in16[k >> 5] |= (uint32_t)(types[i] & 1) << (k & 31);
-                t.out16[k >> 5] |= (uint32_t)((types[i] >> 1) & 1) << (k & 31);
-                chunks += (groups + CLIP_GROUPS - 1) / CLIP_GROUPS;
-                MERLOT_CHECK(chunks < ((uint64_t)1 << 31), MERLOT_ESHAPE, "merlot_clip_by_global_norm: 64 TiB in one call");
-            }
-            t.chunk0[t.count] = (uint32_t)chunks;
-            const int blocks = (int)std::min<uint64_t>(std::max<uint64_t>(chunks, 1), CLIP_BLOCKS);
-            if (pass == 0) {
-                hipLaunchKernelGGL(clip_norm_kernel, dim3(blocks), dim3(256), 0, s, t, part + nparts);
-                nparts += blocks;
-            } else if (clip > 0.f || l == 0) {
-                hipLaunchKernelGGL(clip_scale_kernel, dim3(clip > 0.f ? blocks : 1), dim3(256), 0, s, t, (const double*)part, nparts, clip, l == 0 ? norm : nullptr);
-            }
-            if (int rc = merlot_launch_status("merlot_clip_by_global_norm")) return rc;
+    ClipEntry* table = n > CLIP_TENSORS ? (ClipEntry*)(part + CLIP_BLOCKS) : nullptr;
+    ClipTable t;
+    int count = 0, filled = 0;                           // entries in all, of them in the workspace's table
+    uint64_t chunks = 0;
+    for (int64_t i = 0; i < n; ++i) {
+        if (numel[i] == 0) continue;
+        const int es = types[i] & 1 ? 2 : 4;
+        const uint64_t elements = (uint64_t)numel[i] + ((uint64_t)in[i] & 15) / es;       // (groups start at multiples of 16 bytes)
+        t.e[count - filled] = {(const void*)in[i], clip > 0.f ? (void*)out[i] : nullptr, numel[i], (uint32_t)chunks, types[i]};
+        ++count;
+        chunks += (elements + CLIP_CHUNK - 1) / CLIP_CHUNK;
+        MERLOT_CHECK(chunks < ((uint64_t)1 << 31) && count < (1 << 30), MERLOT_ESHAPE, "merlot_clip_by_global_norm: 64 TiB in one call");
+        if (table && count - filled == CLIP_TENSORS) {
+            hipLaunchKernelGGL(clip_table_kernel, dim3(1), dim3(128), 0, s, t, table + filled, CLIP_TENSORS);
+            filled = count;
         }
     }
-    return MERLOT_OK;
+    if (table && count > filled) hipLaunchKernelGGL(clip_table_kernel, dim3(1), dim3(128), 0, s, t, table + filled, count - filled);
+    const int blocks = (int)std::min<uint64_t>(std::max<uint64_t>(chunks, 1), CLIP_BLOCKS);
+    const dim3 grid(blocks), last(clip > 0.f ? blocks : 1), block(256);
+    if (table) {
+        hipLaunchKernelGGL(clip_norm_table_kernel, grid, block, 0, s, (const ClipEntry*)table, count, (uint32_t)chunks, part);
+        hipLaunchKernelGGL(clip_scale_table_kernel, last, block, 0, s, (const ClipEntry*)table, count, (uint32_t)chunks, (const double*)part, blocks, clip, norm);
+    } else {
+        hipLaunchKernelGGL(clip_norm_kernel, grid, block, 0, s, t, count, (uint32_t)chunks, part);
+        hipLaunchKernelGGL(clip_scale_kernel, last, block, 0, s, t, count, (uint32_t)chunks, (const double*)part, blocks, clip, norm);
+    }
+    return merlot_launch_status("merlot_clip_by_global_norm");
 }

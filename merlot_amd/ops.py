@@ -1070,7 +1070,7 @@ def gemm_f8_blocks(a8, a_scale, b8, b_scale, *, bias=None, out=None, out_dtype=B
 
 class TensorList(object):
     """Many dense f32 / bf16 tensors of one device as ONE operand (global_norm, clip_by_global_norm): checked once, for as long as the tensors stay where they are.
-    Holds references to them; a tensor whose storage has been exchanged since (`t.data = ...`) makes the next use raise."""
+    Keeps their memory alive; a tensor whose storage has been exchanged since (`t.data = ...`) makes the next use raise."""
 
     def __init__(self, tensors):
         import ctypes
@@ -1087,6 +1087,7 @@ class TensorList(object):
             if not t.is_contiguous():
                 raise ValueError(f"tensor {i}: must be contiguous")
         self.device = dev
+        self.memory = [t.detach() for t in self.tensors]      # the storages, whatever becomes of the tensors
         self.shapes = [t.shape for t in self.tensors]
         self.addresses = [t.data_ptr() for t in self.tensors]
         self.ptrs = (ctypes.c_int64 * n)(*self.addresses)
@@ -1097,8 +1098,8 @@ class TensorList(object):
         return len(self.tensors)
 
     def check(self):
-        if [t.data_ptr() for t in self.tensors] != self.addresses or [t.shape for t in self.tensors] != self.shapes:
-            raise ValueError("TensorList: a tensor's storage or shape has changed since the list was made")
+        if list(map(torch.Tensor.data_ptr, self.tensors)) != self.addresses:
+            raise ValueError("TensorList: a tensor's storage has changed since the list was made")
 
 
 def _tensor_list(ts):
@@ -1110,7 +1111,7 @@ def _tensor_list(ts):
 
 def _clip(grads, clip, out):
     import ctypes
-    types = bytes(a | (b << 1) for a, b in zip(grads.bf16, out.bf16))
+    types = bytes(a | (b << 1) for a, b in zip(grads.bf16, out.bf16)) if any(grads.bf16) or any(out.bf16) else bytes(len(grads))
     _here(grads.tensors[0], out.tensors[0])
     n = len(grads)
     norm = torch.empty((), device=grads.device, dtype=F32)
