@@ -73,7 +73,7 @@ def test_clip_refusals_and_overlaps():
         rc, msg = clip(**kw)
         assert rc < 0 and what in msg, (kw, rc, msg)
     q = lib.LIB.query
-    assert q('merlot_clip_workspace_bytes', 1) == q('merlot_clip_workspace_bytes', 128) < q('merlot_clip_workspace_bytes', 129) and q('merlot_clip_workspace_bytes', 0) == 0
+    assert q('merlot_clip_workspace_bytes', 1) == q('merlot_clip_workspace_bytes', 112) < q('merlot_clip_workspace_bytes', 113) and q('merlot_clip_workspace_bytes', 0) == 0
 
 
 def test_python_refusals_need_no_device():
