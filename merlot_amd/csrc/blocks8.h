@@ -15,11 +15,14 @@ __device__ __forceinline__ int block_scale_byte(uint32_t amax_bits, int top) {
 // 2^-e of a scale byte, exactly (bytes 0 ... 247 of finite blocks: the result's own exponent field is 254 - byte)
 __device__ __forceinline__ float block_inverse(int byte) { return __uint_as_float((uint32_t)(254 - byte) << 23); }
 
-// max over each aligned group of G lanes (G = 16 or 32)
+// max over each aligned group of G lanes (G = 16 or 32): rotations inside rows of 16 lanes (data-parallel primitives, no LDS), one exchange between two rows
 template <int G>
 __device__ __forceinline__ uint32_t group_umax(uint32_t m) {
-#pragma unroll
-    for (int o = G / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x128, 0xf, 0xf, true));      // row_ror:8
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x124, 0xf, 0xf, true));      // row_ror:4
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x122, 0xf, 0xf, true));      // row_ror:2
+    m = max(m, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)m, 0x121, 0xf, 0xf, true));      // row_ror:1
+    if constexpr (G == 32) m = max(m, (uint32_t)__shfl_xor((int)m, 16, 64));
     return m;
 }
 

@@ -27,18 +27,25 @@ __global__ __launch_bounds__(256) void quantize_blocks_kernel(const QuantArgs p)
     const T* x = (const T*)p.x + r0 * p.ldx + c0;
     const int rows = (int)min((int64_t)128, p.R - r0), cols = (int)min((int64_t)128, p.C - c0);
     T v[8][8];
-#pragma unroll
-    for (int r = 0; r < 8; ++r) {
-        const int row = r8 * 8 + r, left = cols - c8 * 8;
-        const T* src = x + row * p.ldx + c8 * 8;
+    // every lane loads -- from x's start where its own eight elements do not all exist --, so that the eight rows are in flight together; the others are set right after
+    const int left = cols - c8 * 8;
+    if (p.C >= 8) {
         typedef T vec_t __attribute__((ext_vector_type(8), aligned(WIDE ? 16 : sizeof(T))));
-        if (row < rows && left >= 8) {
-            const vec_t t = *reinterpret_cast<const vec_t*>(src);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+            const int row = r8 * 8 + r;
+            const vec_t t = *reinterpret_cast<const vec_t*>(row < rows && left >= 8 ? x + row * p.ldx + c8 * 8 : (const T*)p.x);
 #pragma unroll
             for (int e = 0; e < 8; ++e) v[r][e] = t[e];
-        } else {
+        }
+    }
+    if (left < 8 || r8 * 8 + 8 > rows) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[r][e] = (row < rows && e < left) ? src[e] : (T)0.f;
+        for (int r = 0; r < 8; ++r) {
+            const int row = r8 * 8 + r;
+            if (row < rows && left >= 8 && p.C >= 8) continue;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[r][e] = row < rows && e < left ? x[row * p.ldx + c8 * 8 + e] : (T)0.f;
         }
     }
     uint32_t rm[8], cm[8];                               // max |x| as bits: non-negative floats order like their bit patterns, infinities and NaN above all numbers

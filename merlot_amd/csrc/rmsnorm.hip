@@ -15,10 +15,10 @@ namespace {
 // VEC consecutive elements at any element alignment (gfx950 loads and stores global dwords at byte alignment): rows of odd width need no path of their own
 template <typename T, int VEC> struct ElemVec { typedef T type __attribute__((ext_vector_type(VEC), aligned(sizeof(T)))); };
 
-// `left`: how many of the VEC elements exist (may be <= 0)
-template <typename T, int VEC>
+// `left`: how many of the VEC elements exist (may be <= 0); FULL: all of them do, the width is a whole number of slabs
+template <typename T, int VEC, bool FULL>
 __device__ __forceinline__ void load_vec(const T* p, int left, float (&v)[VEC]) {
-    if (left >= VEC) {
+    if (FULL || left >= VEC) {
         const typename ElemVec<T, VEC>::type t = *reinterpret_cast<const typename ElemVec<T, VEC>::type*>(p);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[e] = (float)t[e];
@@ -27,9 +27,9 @@ __device__ __forceinline__ void load_vec(const T* p, int left, float (&v)[VEC]) 
         for (int e = 0; e < VEC; ++e) v[e] = e < left ? (float)p[e] : 0.f;
     }
 }
-template <typename T, int VEC>
+template <typename T, int VEC, bool FULL>
 __device__ __forceinline__ void store_vec(T* p, int left, const float (&v)[VEC]) {
-    if (left >= VEC) {
+    if (FULL || left >= VEC) {
         typename ElemVec<T, VEC>::type t;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) t[e] = (T)v[e];
@@ -68,7 +68,7 @@ struct RmsFwdArgs {
     int64_t rows; int H; float eps;
 };
 
-template <typename T, int VEC, int NS, int WPR, bool RES>
+template <typename T, int VEC, int NS, int WPR, bool FULL, bool RES>
 __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwdArgs p) {
     constexpr int RPB = 4 / WPR;                         // rows in flight per workgroup
     __shared__ float red[2][WPR];
@@ -85,13 +85,13 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwdArgs p) {
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             const int c = i * SLAB + c0;
-            load_vec<T, VEC>(x + row * p.ldx + c, H - c, v[i]);
+            load_vec<T, VEC, FULL>(x + row * p.ldx + c, H - c, v[i]);
             if constexpr (RES) {
                 float r[VEC];
-                load_vec<T, VEC>(res + row * p.ldr + c, H - c, r);
+                load_vec<T, VEC, FULL>(res + row * p.ldr + c, H - c, r);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) v[i][e] = (float)(T)(v[i][e] + r[e]);
-                store_vec<T, VEC>((T*)p.h + row * H + c, H - c, v[i]);
+                store_vec<T, VEC, FULL>((T*)p.h + row * H + c, H - c, v[i]);
             }
 #pragma unroll
             for (int e = 0; e < VEC; ++e) ss += v[i][e] * v[i][e];
@@ -103,17 +103,17 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwdArgs p) {
         for (int i = 0; i < NS; ++i) {
             const int c = i * SLAB + c0;
             float g[VEC];
-            load_vec<float, VEC>(p.gamma + c, H - c, g);
+            load_vec<float, VEC, FULL>(p.gamma + c, H - c, g);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[i][e] = v[i][e] * rstd * g[e];
-            if (p.y) store_vec<T, VEC>((T*)p.y + row * H + c, H - c, v[i]);
+            if (p.y) store_vec<T, VEC, FULL>((T*)p.y + row * H + c, H - c, v[i]);
             if (p.y8) {                                  // from the unrounded y: ONE rounding between it and the 8-bit value
                 uint32_t m = 0;
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) m = max(m, __float_as_uint(v[i][e]) & 0x7fffffffu);
                 m = group_umax<128 / VEC>(m);
                 const int byte = block_scale_byte(m, E4M3_TOP);
-                if (c < p.ld8) {
+                if (FULL || c < p.ld8) {
                     store_codes<0, VEC>(p.y8 + row * p.ld8 + c, v[i], byte);
                     if ((c & 127) == 0) p.s8[row * p.lds8 + (c >> 7)] = (uint8_t)byte;
                 }
@@ -132,7 +132,7 @@ struct RmsBwdArgs {
     int64_t rows; int H;
 };
 
-template <typename T, int VEC, int NS, int WPR>
+template <typename T, int VEC, int NS, int WPR, bool FULL>
 __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdArgs p) {
     constexpr int RPB = 4 / WPR;
     constexpr int SLAB = WPR * 64 * VEC;
@@ -158,9 +158,9 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdArgs p) {
         for (int i = 0; i < NS; ++i) {
             const int c = i * SLAB + c0;
             float g[VEC];
-            load_vec<T, VEC>(h + row * p.ldh + c, H - c, n[i]);
-            load_vec<T, VEC>(dy + row * p.lddy + c, H - c, t[i]);
-            load_vec<float, VEC>(p.gamma + c, H - c, g);
+            load_vec<T, VEC, FULL>(h + row * p.ldh + c, H - c, n[i]);
+            load_vec<T, VEC, FULL>(dy + row * p.lddy + c, H - c, t[i]);
+            load_vec<float, VEC, FULL>(p.gamma + c, H - c, g);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 n[i][e] *= rs;
@@ -178,11 +178,11 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdArgs p) {
             for (int e = 0; e < VEC; ++e) o[e] = rs * (t[i][e] - n[i][e] * c1);
             if (dres) {
                 float r[VEC];
-                load_vec<T, VEC>(dres + row * p.lddr + c, H - c, r);
+                load_vec<T, VEC, FULL>(dres + row * p.lddr + c, H - c, r);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) o[e] += r[e];
             }
-            store_vec<T, VEC>((T*)p.dx + row * H + c, H - c, o);
+            store_vec<T, VEC, FULL>((T*)p.dx + row * H + c, H - c, o);
         }
     }
     // the workgroup's rows together, in a fixed order; the partial sums are added up by rms_dgamma_kernel (no atomics: the same call gives the same bits)
@@ -202,7 +202,7 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdArgs p) {
                     p.part[(int64_t)blockIdx.x * H + i * SLAB + k] = s;
                 }
         } else {
-            store_vec<float, VEC>(p.part + (int64_t)blockIdx.x * H + c, H - c, dg[i]);
+            store_vec<float, VEC, FULL>(p.part + (int64_t)blockIdx.x * H + c, H - c, dg[i]);
         }
     }
 }
@@ -229,16 +229,22 @@ constexpr int RMS_MAX_H = 16384;
 
 // (VEC, NS, WPR) by width: one wave and 8 features per lane up to 2 048, but 4 per lane where 8 would leave half of the last slab's lanes idle (ceil(H / 256)
 // odd, up to 768); four waves above
-#define RMS_DISPATCH(H, CALL)                                                                                   \
+#define RMS_WIDTH(H, V, N, W, ...)                                                                             \
     do {                                                                                                        \
-        if ((H) <= 256) { constexpr int VEC = 4, NS = 1, WPR = 1; CALL; }                                       \
-        else if ((H) <= 512) { constexpr int VEC = 8, NS = 1, WPR = 1; CALL; }                                  \
-        else if ((H) <= 768) { constexpr int VEC = 4, NS = 3, WPR = 1; CALL; }                                  \
-        else if ((H) <= 1024) { constexpr int VEC = 8, NS = 2, WPR = 1; CALL; }                                 \
-        else if ((H) <= 2048) { constexpr int VEC = 8, NS = 4, WPR = 1; CALL; }                                 \
-        else if ((H) <= 4096) { constexpr int VEC = 8, NS = 2, WPR = 4; CALL; }                                 \
-        else if ((H) <= 8192) { constexpr int VEC = 8, NS = 4, WPR = 4; CALL; }                                 \
-        else { constexpr int VEC = 8, NS = 8, WPR = 4; CALL; }                                                  \
+        constexpr int VEC = V, NS = N, WPR = W;                                                                 \
+        if ((H) == VEC * 64 * WPR * NS) { constexpr bool FULL = true; __VA_ARGS__; }                                   \
+        else { constexpr bool FULL = false; __VA_ARGS__; }                                                             \
+    } while (0)
+#define RMS_DISPATCH(H, ...)                                                                                   \
+    do {                                                                                                        \
+        if ((H) <= 256) RMS_WIDTH(H, 4, 1, 1, __VA_ARGS__);                                                            \
+        else if ((H) <= 512) RMS_WIDTH(H, 8, 1, 1, __VA_ARGS__);                                                       \
+        else if ((H) <= 768) RMS_WIDTH(H, 4, 3, 1, __VA_ARGS__);                                                       \
+        else if ((H) <= 1024) RMS_WIDTH(H, 8, 2, 1, __VA_ARGS__);                                                      \
+        else if ((H) <= 2048) RMS_WIDTH(H, 8, 4, 1, __VA_ARGS__);                                                      \
+        else if ((H) <= 4096) RMS_WIDTH(H, 8, 2, 4, __VA_ARGS__);                                                      \
+        else if ((H) <= 8192) RMS_WIDTH(H, 8, 4, 4, __VA_ARGS__);                                                      \
+        else RMS_WIDTH(H, 8, 8, 4, __VA_ARGS__);                                                                       \
     } while (0)
 
 int rms_rows_per_block(int H) { return H <= 2048 ? 4 : 1; }
@@ -253,9 +259,9 @@ void rms_fwd_launch(const RmsFwdArgs& a, hipStream_t s) {
     const int64_t nb = (a.rows + rms_rows_per_block(a.H) - 1) / rms_rows_per_block(a.H);
     const dim3 grid((unsigned)(nb < 4096 ? nb : 4096)), block(256);
     if (a.res)
-        RMS_DISPATCH(a.H, hipLaunchKernelGGL((rms_fwd_kernel<T, VEC, NS, WPR, true>), grid, block, 0, s, a));
+        RMS_DISPATCH(a.H, hipLaunchKernelGGL((rms_fwd_kernel<T, VEC, NS, WPR, FULL, true>), grid, block, 0, s, a));
     else
-        RMS_DISPATCH(a.H, hipLaunchKernelGGL((rms_fwd_kernel<T, VEC, NS, WPR, false>), grid, block, 0, s, a));
+        RMS_DISPATCH(a.H, hipLaunchKernelGGL((rms_fwd_kernel<T, VEC, NS, WPR, FULL, false>), grid, block, 0, s, a));
 }
 
 }  // namespace
@@ -292,8 +298,8 @@ extern "C" int merlot_rms_bwd(const void* dy, int64_t lddy, int is_f32, const vo
     const RmsBwdArgs a = {dy, lddy, h, ldh, rstd, gamma, dres, lddr, dx, (float*)workspace, rows, H};
     hipStream_t s = (hipStream_t)stream;
     const dim3 grid(nb), block(256);
-    if (is_f32) RMS_DISPATCH(H, hipLaunchKernelGGL((rms_bwd_kernel<float, VEC, NS, WPR>), grid, block, 0, s, a));
-    else RMS_DISPATCH(H, hipLaunchKernelGGL((rms_bwd_kernel<bf16, VEC, NS, WPR>), grid, block, 0, s, a));
+    if (is_f32) RMS_DISPATCH(H, hipLaunchKernelGGL((rms_bwd_kernel<float, VEC, NS, WPR, FULL>), grid, block, 0, s, a));
+    else RMS_DISPATCH(H, hipLaunchKernelGGL((rms_bwd_kernel<bf16, VEC, NS, WPR, FULL>), grid, block, 0, s, a));
     if (int rc = merlot_launch_status("merlot_rms_bwd")) return rc;
     hipLaunchKernelGGL(rms_dgamma_kernel, dim3((H + 63) / 64), dim3(1024), 0, s, (const float*)workspace, dgamma, nb, H);
     return merlot_launch_status("merlot_rms_bwd");
