@@ -74,6 +74,7 @@ __device__ __forceinline__ void wait_step() { asm volatile("s_waitcnt vmcnt(%0) 
 // Tile 128 x BN, four waves (64 x 128 each for BN 256, 64 x 64 for BN 128), K-steps of 64, three step buffers filled by LDS-DMA two to three steps ahead, one
 // barrier per step.  Two workgroups share a CU (72 + 6 KiB of LDS, 256 registers): while one waits, loads or stores its tile, the other multiplies.
 // OUT: 0 bf16, 1 fp32, 2 fp32 partial products of a split reduction.  EXACT: through bf16 fragments (see above).
+constexpr int direct_unroll(int mf) { return mf <= 2 ? 4 : 2; }       // blocks in flight per wave of blocks_direct_kernel
 constexpr int SCALE_BLOCKS = 16;                         // blocks of 128 whose scale bytes lie in LDS at a time (16 bytes per row)
 
 template <int FA, int BN, int OUT, bool EXACT>
@@ -289,7 +290,6 @@ constexpr int WIDE_LDS = WIDE_SLAB + 4 * 4096;           // two K-tiles, 16 bloc
 template <int FA, bool LINES>
 __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p) {
 #ifdef __HIP_DEVICE_COMPILE__
-    typedef bf16 T;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hi = lane >> 5, l31 = lane & 31, wm = wave >> 1, wn = wave & 1;
@@ -557,6 +557,96 @@ __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p)
 #endif
 }
 
+// Few rows, or little work: 16 NF columns x 16 MF rows per workgroup, the reduction dealt out block by block to its eight waves and joined once, in wave order, through
+// LDS.  The operands go straight from memory to the registers (16 rows x 128 bytes: whole lines), every load of UNROLL blocks in flight at once: what bounds such a
+// product is one round trip to memory, and the operands' way through the L2.
+template <int FA, int MF, int NF, typename T>
+__global__ __launch_bounds__(512) void blocks_direct_kernel(const BlocksArgs p) {
+#ifdef __HIP_DEVICE_COMPILE__
+    constexpr bool EXACT = sizeof(T) == 4;
+    constexpr int UNROLL = direct_unroll(MF);
+    __shared__ f32x4 part[8][MF * NF][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), l15 = lane & 15, quarter = lane >> 4;
+    const int64_t n0 = (int64_t)blockIdx.x * (16 * NF), m0 = (int64_t)blockIdx.y * (16 * MF);
+    const int64_t K = (int64_t)p.nk * 128;
+    const int rows_a = (int)min((int64_t)(16 * MF), p.M - m0), rows_b = (int)min((int64_t)(16 * NF), p.N - n0);
+    const __amdgpu_buffer_rsrc_t ra = rows_rsrc(p.A, m0, rows_a, p.lda, K), rb = rows_rsrc(p.B, n0, rows_b, p.ldb, K);
+    const __amdgpu_buffer_rsrc_t rsa = rows_rsrc(p.sa, m0, rows_a, p.ldsa, p.nk), rsb = rows_rsrc(p.sb, n0, rows_b, p.ldsb, p.nk);
+    f32x4 acc[MF][NF];
+#pragma unroll
+    for (int f = 0; f < MF; ++f)
+#pragma unroll
+        for (int g = 0; g < NF; ++g) acc[f][g] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const unsigned oa = (unsigned)(l15 * p.lda) + quarter * 32, ob = (unsigned)(l15 * p.ldb) + quarter * 32, osa = (unsigned)(l15 * p.ldsa), osb = (unsigned)(l15 * p.ldsb);
+    for (int kb = wave; kb < p.nk; kb += 8 * UNROLL) {
+        i32x4 a[UNROLL][MF][2], b[UNROLL][NF][2];
+        int xa[UNROLL][MF], xb[UNROLL][NF];
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            const int k = kb + 8 * u;                    // (blocks past the last one: zeros times 2^0, without a trip to memory)
+            const bool there = k < p.nk;
+#pragma unroll
+            for (int g = 0; g < NF; ++g) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    b[u][g][h] = there ? __builtin_amdgcn_raw_buffer_load_b128(rb, ob + (unsigned)(g * 16 * p.ldb) + h * 16, k * 128, 0) : i32x4{0, 0, 0, 0};
+                xb[u][g] = there ? __builtin_amdgcn_raw_buffer_load_b8(rsb, osb + (unsigned)(g * 16 * p.ldsb), k, 0) : 127;
+            }
+#pragma unroll
+            for (int f = 0; f < MF; ++f) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    a[u][f][h] = there ? __builtin_amdgcn_raw_buffer_load_b128(ra, oa + (unsigned)(f * 16 * p.lda) + h * 16, k * 128, 0) : i32x4{0, 0, 0, 0};
+                xa[u][f] = there ? __builtin_amdgcn_raw_buffer_load_b8(rsa, osa + (unsigned)(f * 16 * p.ldsa), k, 0) : 127;
+            }
+        }
+#pragma unroll
+        for (int u = 0; u < UNROLL; ++u) {
+            if constexpr (!EXACT) {
+#pragma unroll
+                for (int f = 0; f < MF; ++f)
+#pragma unroll
+                    for (int g = 0; g < NF; ++g)
+                        acc[f][g] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(__builtin_shufflevector(b[u][g][0], b[u][g][1], 0, 1, 2, 3, 4, 5, 6, 7),
+                                                                                     __builtin_shufflevector(a[u][f][0], a[u][f][1], 0, 1, 2, 3, 4, 5, 6, 7), acc[f][g], 0, FA, 0,
+                                                                                     xb[u][g], 0, xa[u][f]);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    bf16x8 wb[NF];
+#pragma unroll
+                    for (int g = 0; g < NF; ++g) wb[g] = widen<0>(b[u][g][q >> 1][2 * (q & 1)], b[u][g][q >> 1][2 * (q & 1) + 1], scale_value(xb[u][g] & 255));
+#pragma unroll
+                    for (int f = 0; f < MF; ++f) {
+                        const bf16x8 wa = widen<FA>(a[u][f][q >> 1][2 * (q & 1)], a[u][f][q >> 1][2 * (q & 1) + 1], scale_value(xa[u][f] & 255));
+#pragma unroll
+                        for (int g = 0; g < NF; ++g) acc[f][g] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wb[g], wa, acc[f][g], 0, 0, 0);
+                    }
+                }
+            }
+        }
+    }
+#pragma unroll
+    for (int f = 0; f < MF; ++f)
+#pragma unroll
+        for (int g = 0; g < NF; ++g) part[wave][f * NF + g][lane] = acc[f][g];
+    __syncthreads();
+    // lane <-> row (lane & 15) of A, register r <-> column 4 (lane >> 4) + r
+    if (wave < MF * NF) {
+        f32x4 s = part[0][wave][lane];
+#pragma unroll
+        for (int w = 1; w < 8; ++w) s += part[w][wave][lane];
+        const int64_t m = m0 + wave / NF * 16 + l15, n = n0 + wave % NF * 16 + quarter * 4, left = p.N - n;
+        if (m < p.M && left > 0) {
+            T __attribute__((ext_vector_type(4))) o;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) o[e] = (T)(s[e] + (p.bias && e < left ? p.bias[n + e] : 0.f));
+            store_out<T, 4>((T*)p.C + m * p.ldc + n, left, o, p.accumulate != 0);
+        }
+    }
+#endif
+}
+
 // the splits' partial products together, in their order, + bias
 template <typename T>
 __global__ __launch_bounds__(256) void blocks_fold_kernel(const BlocksArgs p, int splits) {
@@ -581,21 +671,30 @@ __global__ __launch_bounds__(256) void blocks_fold_kernel(const BlocksArgs p, in
 
 struct BlocksPlan { int bm, bn, splits, nk_split; };
 
+// Straight from memory where every wave has its whole share of the reduction in flight at once (twice at most, with 16 rows) and the operands' way through the L2 --
+// workgroups x (rows + columns) each -- stays short (us, 128-row tiles : direct): 1 x 2304 x 768 6.8 : 3.0, 32 x 4096 x 4096 12.1 : 10.8, 700 x 500 x 1024 9.3 : 6.5,
+// 512 x 1024 x 1024 8.5 : 6.2, 100 x 4096 x 2048 12.1 : 9.7; but 16 x 50370 x 768 10.9 : 17.1, 64 x 4096 x 4096 13.3 : 19.3, 1000 x 1000 x 1024 9.0 : 11.1.
 // bf16 outputs take 256 x 256 tiles where those fill the 256 CUs and the reduction is long enough to pay for an epilogue nobody covers (us, 128 x 256 tiles : 256 x 256):
 //   101376 x 2304 x 384 139 : 138, x 512 161 : 139, x 768 224 : 200; 65536 x 768 x 768 55 : 49; 32768 x 4096 x 1024 159 : 142; 8192^3 513 : 400
 // With rows of C that start inside a 64-byte sector their 128-byte row pieces are written as parts of lines, past the caches or not: 101376 x 2296 x 768 225 : 306, and only a
 // long reduction hides it (30000 x 2296 x 2048 163 : 147, x 4096 297 : 254; 4099 x 50370 x 2048 467 : 476).  fp32 outputs gain nothing (the bf16 matrix instructions are the bound either way).
-// 128 x 256 where those fill the CUs twice; otherwise narrow tiles, and a long reduction is split until there are about 512 workgroups, at least eight blocks (16 steps) each
+// 128 x 256 where those fill the CUs twice; otherwise the reduction is split, or narrow tiles.
 BlocksPlan blocks_plan(int64_t M, int64_t N, int64_t K, bool out_bf16, bool whole_lines) {
     const int64_t tm = (M + 127) / 128, nk = K / 128;
+    // straight from memory: 16 x 16, 32 x 16 or 64 x 32 outputs per workgroup
+    const int mf = M <= 16 ? 1 : M <= 32 ? 2 : 4, nf = mf == 4 ? 2 : 1;
+    if (nk <= 8 * direct_unroll(mf) * (mf == 1 ? 2 : 1) && (M + 16 * mf - 1) / (16 * mf) * ((N + 16 * nf - 1) / (16 * nf)) * (mf + nf) <= 3000) return {16 * mf, 16 * nf, 1, (int)nk};
     if (out_bf16 && nk >= (whole_lines ? 4 : 16) && ((M + 255) / 256) * ((N + 255) / 256) >= 256) return {256, 256, 1, (int)nk};
     if (N > 128 && tm * ((N + 255) / 256) >= 512) return {128, 256, 1, (int)nk};
-    const int64_t tiles = tm * ((N + 127) / 128);
-    int64_t s = 512 / tiles;
-    if (s > nk / 8) s = nk / 8;
-    if (s < 2) return {128, 128, 1, (int)nk};
-    const int64_t per = ((nk + s - 1) / s + 3) / 4 * 4;
-    return {128, 128, (int)((nk + per - 1) / per), (int)per};
+    // a long reduction: split until there are about 512 workgroups, 24 blocks each at least with the wide tile, eight with the narrow one (fp32, narrow : wide:
+    // 4096 x 1024 x 32768 251 : 236, 2304 x 768 x 101376 370 : 328; but 18 wide tiles, 768 x 768 x 65536, 92 : 102)
+    for (int bn = N > 128 ? 256 : 128; bn >= 128; bn -= 128) {
+        const int64_t tiles = tm * ((N + bn - 1) / bn), s = min(512 / tiles, nk / (bn == 256 ? 24 : 8));
+        if (s < 2 || (bn == 256 && tiles < 32)) continue;
+        const int64_t per = ((nk + s - 1) / s + 3) / 4 * 4;
+        return {128, bn, (int)((nk + per - 1) / per), (int)per};
+    }
+    return {128, 128, 1, (int)nk};
 }
 
 template <int FA, bool LINES>
@@ -606,20 +705,26 @@ int blocks_wide_launch(const BlocksArgs& p, hipStream_t s) {
     return MERLOT_OK;
 }
 
+template <int FA, typename T>
+void blocks_direct_launch(const BlocksArgs& p, int bm, hipStream_t s) {
+    const dim3 grid(p.ntn, p.ntm), block(512);
+    if (bm == 16) hipLaunchKernelGGL((blocks_direct_kernel<FA, 1, 1, T>), grid, block, 0, s, p);
+    else if (bm == 32) hipLaunchKernelGGL((blocks_direct_kernel<FA, 2, 1, T>), grid, block, 0, s, p);
+    else hipLaunchKernelGGL((blocks_direct_kernel<FA, 4, 2, T>), grid, block, 0, s, p);
+}
+
 template <int FA, int BN>
 void blocks_launch(const BlocksArgs& p, int splits, bool out_f32, hipStream_t s) {
     const dim3 grid(p.ntm * p.ntn, splits), block(256);
     if (splits > 1) {
-        if constexpr (BN == 128) {
-            const int64_t work = p.M * ((p.N + 3) / 4);
-            const dim3 fold((unsigned)min((int64_t)4096, (work + 255) / 256));
-            if (out_f32) {
-                hipLaunchKernelGGL((blocks_gemm_kernel<FA, BN, 2, true>), grid, block, 0, s, p);
-                hipLaunchKernelGGL((blocks_fold_kernel<float>), fold, block, 0, s, p, splits);
-            } else {
-                hipLaunchKernelGGL((blocks_gemm_kernel<FA, BN, 2, false>), grid, block, 0, s, p);
-                hipLaunchKernelGGL((blocks_fold_kernel<bf16>), fold, block, 0, s, p, splits);
-            }
+        const int64_t work = p.M * ((p.N + 3) / 4);
+        const dim3 fold((unsigned)min((int64_t)4096, (work + 255) / 256));
+        if (out_f32) {
+            hipLaunchKernelGGL((blocks_gemm_kernel<FA, BN, 2, true>), grid, block, 0, s, p);
+            hipLaunchKernelGGL((blocks_fold_kernel<float>), fold, block, 0, s, p, splits);
+        } else {
+            hipLaunchKernelGGL((blocks_gemm_kernel<FA, BN, 2, false>), grid, block, 0, s, p);
+            hipLaunchKernelGGL((blocks_fold_kernel<bf16>), fold, block, 0, s, p, splits);
         }
     } else if (out_f32) {
         hipLaunchKernelGGL((blocks_gemm_kernel<FA, BN, 1, true>), grid, block, 0, s, p);
@@ -656,7 +761,10 @@ extern "C" int merlot_gemm_f8_blocks(const void* A8, int64_t lda, int fmt_a, con
     const BlocksArgs p = {(const uint8_t*)A8, (const uint8_t*)B8, scale_a, scale_b, lda, ldb, ld_scale_a, ld_scale_b, C, ldc, bias, (float*)workspace, M, N,
                           (int)(K / 128), plan.nk_split, (int)ntm, (int)ntn, accumulate, (unsigned)(((uint64_t)1 << 32) / (4 * (uint64_t)ntn))};
     hipStream_t s = (hipStream_t)stream;
-    if (plan.bm == 256) {
+    if (plan.bn <= 64) {
+        if (out_f32) fmt_a == 0 ? blocks_direct_launch<0, float>(p, plan.bm, s) : blocks_direct_launch<1, float>(p, plan.bm, s);
+        else fmt_a == 0 ? blocks_direct_launch<0, bf16>(p, plan.bm, s) : blocks_direct_launch<1, bf16>(p, plan.bm, s);
+    } else if (plan.bm == 256) {
         const int rc = fmt_a == 0 ? (whole_lines ? blocks_wide_launch<0, true>(p, s) : blocks_wide_launch<0, false>(p, s))
                                   : (whole_lines ? blocks_wide_launch<1, true>(p, s) : blocks_wide_launch<1, false>(p, s));
         if (rc != MERLOT_OK) return rc;

@@ -46,7 +46,7 @@ def test_block_refusals():
     ok = dict(a=P, lda=256, fa=0, sa=P, lsa=4, b=P, ldb=256, sb=P, lsb=4, c=P, ldc=300, M=5000, N=300, K=256, f=0, acc=0, bias=None, ws=None, wsb=0, st=None)
     for kw, what in ((dict(a=None), 'null'), (dict(sb=None), 'null'), (dict(M=0), 'size'), (dict(N=0), 'size'), (dict(K=250), 'size'), (dict(K=0), 'size'), (dict(fa=2), 'fmt_a'),
                      (dict(acc=1), 'accumulation'), (dict(lda=128), 'leading'), (dict(ldc=299), 'leading'), (dict(lda=264), 'aligned'), (dict(b=P + 8), 'aligned'),
-                     (dict(lsa=1), 'scale'), (dict(lsb=6), 'scale'), (dict(sa=P + 2), 'scale'), (dict(M=5, K=8192, lda=8192, ldb=8192, lsa=64, lsb=64), 'workspace')):
+                     (dict(lsa=1), 'scale'), (dict(lsb=6), 'scale'), (dict(sa=P + 2), 'scale'), (dict(M=200, K=8192, lda=8192, ldb=8192, lsa=64, lsb=64), 'workspace')):
         rc, msg = _call('merlot_gemm_f8_blocks', *{**ok, **kw}.values())
         assert rc < 0 and what in msg, (kw, rc, msg)
 

@@ -95,7 +95,7 @@ def _operand(rows, K, fmt, seed, tile=1, whole=False):
 MS, NS = [1, 2, 7, 16, 17, 31, 32, 33, 64, 65, 127, 128, 129, 256, 257, 300, 513], [1, 2, 5, 16, 64, 100, 129, 255, 256, 500, 770]
 
 
-@pytest.mark.parametrize('K', [128, 256, 384, 640, 1024, 1152, 4224])
+@pytest.mark.parametrize('K', [128, 256, 384, 640, 1024, 1152, 2048, 4224])
 @pytest.mark.parametrize('M', MS)
 def test_product_of_whole_numbers_is_exact(M, K):
     """sums under 2^24: 64 * 16 * 4224 < 2^23"""
