@@ -88,7 +88,7 @@ class _Lib(object):
         return getattr(self.load(), name)(*args)
 
     def call(self, name, *args):
-        dll = self.load()
+        dll = self._dll or self.load()
         rc = getattr(dll, name)(*args)
         if rc != 0:
             msg = dll.merlot_last_error()

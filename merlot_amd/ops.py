@@ -917,18 +917,18 @@ def _operands(*operands):
 
 def _rows(t, name):
     """(2-D view, row stride): any leading dims where they collapse without a copy; rows may be further apart than they are long, not nearer"""
-    if t.dim() == 0:
-        raise ValueError(f"{name}: expected at least one dimension")
     if t.dim() != 2:
         try:
             t = t.view(-1, t.shape[-1]) if t.numel() else t.reshape(0, t.shape[-1])
         except RuntimeError:
             raise ValueError(f"{name}: leading dimensions do not collapse into rows without a copy") from None
-    if t.shape[0] <= 1:
-        return t, t.shape[1]
-    if t.stride(0) < t.shape[1]:
-        raise ValueError(f"{name}: rows overlap (stride {t.stride(0)}, {t.shape[1]} columns)")
-    return t, t.stride(0)
+    rows, cols = t.shape
+    if rows <= 1:
+        return t, cols
+    ld = t.stride(0)
+    if ld < cols:
+        raise ValueError(f"{name}: rows overlap (stride {ld}, {cols} columns)")
+    return t, ld
 
 
 def _scales8(rows, cols, like):
@@ -963,8 +963,8 @@ def rms_norm_fwd(x, gamma, *, residual=None, out=True, q8=False, save_rstd=True,
         y8 = x.new_empty((rows, (H + 127) // 128 * 128), dtype=FP8)
         s8 = _scales8(rows, H, x)
     if rows:
-        call('merlot_rms_fwd', _p(x2), ldx, 1 if x.dtype == F32 else 0, _p(r2), ldr, _p(gamma), _p(h), _p(y), _p(rstd), _p(y8), y8.shape[1] if q8 else 0,
-             _p(s8), (s8.shape[1] + 3) // 4 * 4 if q8 else 0, rows, H, float(eps), _stream())
+        call('merlot_rms_fwd', x2.data_ptr(), ldx, 1 if x.dtype is F32 else 0, _p(r2), ldr, gamma.data_ptr(), _p(h), _p(y), _p(rstd), _p(y8),
+             (H + 127) // 128 * 128, _p(s8), (H + 511) // 512 * 4, rows, H, eps, _stream())
     return y, h, rstd, y8, s8
 
 
@@ -1017,8 +1017,8 @@ def quantize_blocks(x, fmt=F8_E4M3, *, tile=1, rows=True, transpose=False):
     if transpose:
         qt, st = x.new_empty((C, (R + 127) // 128 * 128), dtype=dt), _scales8(C, R, x)
     if R:
-        call('merlot_quantize_blocks', _p(x2), ldx, 1 if x.dtype == F32 else 0, R, C, int(fmt), int(tile), _p(q), q.shape[1] if rows else 0, _p(s),
-             (s.shape[1] + 3) // 4 * 4 if rows else 0, _p(qt), qt.shape[1] if transpose else 0, _p(st), (st.shape[1] + 3) // 4 * 4 if transpose else 0, _stream())
+        call('merlot_quantize_blocks', x2.data_ptr(), ldx, 1 if x.dtype is F32 else 0, R, C, fmt, tile, _p(q), (C + 127) // 128 * 128, _p(s), (C + 511) // 512 * 4,
+             _p(qt), (R + 127) // 128 * 128, _p(st), (R + 511) // 512 * 4, _stream())
     return (q, s, qt, st) if transpose else (q, s)
 
 
@@ -1051,14 +1051,17 @@ def gemm_f8_blocks(a8, a_scale, b8, b_scale, *, bias=None, out=None, out_dtype=B
         if out_dtype not in (BF16, F32):
             raise ValueError(f"out_dtype: expected bf16 or f32, got {out_dtype}")
         out = a8.new_empty((M, N), dtype=out_dtype)
-    if out.dtype not in (BF16, F32) or out.shape != (M, N):
-        raise ValueError(f"out: expected bf16 or f32 [{M}, {N}], got {out.dtype} {tuple(out.shape)}")
-    if accumulate and out.dtype != F32:
-        raise ValueError("gemm_f8_blocks: accumulate needs an f32 out")
+        ldc = N
+    else:
+        if out.dtype not in (BF16, F32) or out.shape != (M, N):
+            raise ValueError(f"out: expected bf16 or f32 [{M}, {N}], got {out.dtype} {tuple(out.shape)}")
+        if accumulate and out.dtype != F32:
+            raise ValueError("gemm_f8_blocks: accumulate needs an f32 out")
+        if M and N:
+            _operands((out, out.dtype, 'out'))
+            _, ldc = _rows(out, 'out')
     if M == 0 or N == 0:
         return out
-    _operands((out, out.dtype, 'out'))
-    _, ldc = _rows(out, 'out')
     nbytes = LIB.query('merlot_gemm_f8_blocks_workspace_bytes', M, N, K)
     ws = a8.new_empty(nbytes // 4, dtype=F32) if nbytes else None   # caller-owned partial products of a split reduction
 
