@@ -496,10 +496,12 @@ __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p)
         };
         auto round = [&](auto uc) __attribute__((always_inline)) {
             constexpr int U = decltype(uc)::value, I = U & 3, J = (U >> 2) * 2;           // column halves outside: each half's bias is read once
+            f32x16 &s0 = acc[I][J], &s1 = acc[I][J + 1];
+            asm volatile("" : "+a"(s0), "+a"(s1));       // fetched from the accumulation registers here, not all sums at the loop's end
 #pragma unroll
             for (int k = 0; k < 8; ++k)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[k][e] = (bf16)(acc[I][J + (k >> 2)][4 * (k & 3) + e] + bias[k][e]);
+                for (int e = 0; e < 4; ++e) o[k][e] = (bf16)((k < 4 ? s0 : s1)[4 * (k & 3) + e] + bias[k][e]);
         };
         auto write = [&]() __attribute__((always_inline)) {
 #pragma unroll
