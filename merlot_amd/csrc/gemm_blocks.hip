@@ -392,11 +392,14 @@ __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p)
     auto half = [&](auto pc, auto firstc, auto fetchc, unsigned next, int into) __attribute__((always_inline)) {
         constexpr int P = decltype(pc)::value;
         constexpr bool FIRST = decltype(firstc)::value, FETCH = decltype(fetchc)::value;
-        // sixteen slots of one matrix instruction (64 cycles), two reads (the first eight) and one fetch
+        // sixteen slots of one matrix instruction (64 cycles): one read and one fetch in half 1; in half 0 two reads in each of the first eight, so that they have returned
+        // where the barrier behind the half asks for it
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
             const int i = k & 3, j = k >> 2;
-            if (k < 8) {
+            if (P == 1) {
+                read_chunk(std::integral_constant<int, P ^ 1>{}, k, next);
+            } else if (k < 8) {
                 read_chunk(std::integral_constant<int, P ^ 1>{}, 2 * k, next);
                 read_chunk(std::integral_constant<int, P ^ 1>{}, 2 * k + 1, next);
             }
@@ -747,7 +750,8 @@ extern "C" int merlot_gemm_f8_blocks(const void* A8, int64_t lda, int fmt_a, con
                                      const uint8_t* scale_b, int64_t ld_scale_b, void* C, int64_t ldc, int64_t M, int64_t N, int64_t K, int out_f32,
                                      int accumulate, const float* bias, void* workspace, int64_t workspace_bytes, merlot_stream_t stream) {
     MERLOT_CHECK(A8 && B8 && scale_a && scale_b && C, MERLOT_ESHAPE, "merlot_gemm_f8_blocks: null operand");
-    MERLOT_CHECK(M > 0 && N > 0 && K > 0 && K % 128 == 0 && K < ((int64_t)1 << 31), MERLOT_ESHAPE, "merlot_gemm_f8_blocks: bad size (K must be a multiple of 128)");
+    MERLOT_CHECK(M > 0 && N > 0 && K > 0 && K % 128 == 0 && M < ((int64_t)1 << 31) - 256 && N < ((int64_t)1 << 31) - 256, MERLOT_ESHAPE,
+                 "merlot_gemm_f8_blocks: bad size (K must be a multiple of 128)");
     MERLOT_CHECK(fmt_a == 0 || fmt_a == 1, MERLOT_EDTYPE, "merlot_gemm_f8_blocks: fmt_a must be 0 (e4m3) or 1 (e5m2)");
     MERLOT_CHECK(!accumulate || out_f32, MERLOT_EDTYPE, "merlot_gemm_f8_blocks: accumulation needs an fp32 output");
     MERLOT_CHECK(lda >= K && ldb >= K && ldc >= N && lda < (1 << 22) && ldb < (1 << 22), MERLOT_ESHAPE, "merlot_gemm_f8_blocks: bad leading dimension");
@@ -759,7 +763,7 @@ extern "C" int merlot_gemm_f8_blocks(const void* A8, int64_t lda, int fmt_a, con
     const BlocksPlan plan = blocks_plan(M, N, K, !out_f32, whole_lines);
     MERLOT_CHECK(plan.splits == 1 || (workspace && workspace_bytes >= (int64_t)plan.splits * M * N * 4), MERLOT_ESHAPE, "merlot_gemm_f8_blocks: workspace too small");
     const int64_t ntm = (M + plan.bm - 1) / plan.bm, ntn = (N + plan.bn - 1) / plan.bn;
-    MERLOT_CHECK(ntm * ntn < ((int64_t)1 << 31), MERLOT_ESHAPE, "merlot_gemm_f8_blocks: too many tiles");
+    MERLOT_CHECK(ntm * ntn < ((int64_t)1 << 24), MERLOT_ESHAPE, "merlot_gemm_f8_blocks: too many tiles");
     const BlocksArgs p = {(const uint8_t*)A8, (const uint8_t*)B8, scale_a, scale_b, lda, ldb, ld_scale_a, ld_scale_b, C, ldc, bias, (float*)workspace, M, N,
                           (int)(K / 128), plan.nk_split, (int)ntm, (int)ntn, accumulate, (unsigned)(((uint64_t)1 << 32) / (4 * (uint64_t)ntn))};
     hipStream_t s = (hipStream_t)stream;
