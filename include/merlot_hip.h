@@ -574,6 +574,7 @@ int merlot_quantize_blocks(const void* x, int64_t ldx, int x_f32, int64_t R, int
  * writes them, A8 e4m3 (fmt_a 0) or e5m2 (1), B8 e4m3; K % 128 == 0, M and N any; operand rows 16-byte, scale rows 4-byte aligned (leading dimensions too) and
  * read in whole words of 4 bytes.  fp32 accumulators; an f32 C is good to fp32 (the codes go through the bf16 matrix instruction, exactly), a bf16 C comes from the
  * 8-bit instruction, which keeps 13 bits below the largest of each eight products.  C bf16 or f32 (out_f32; accumulate adds into C before the one rounding), ldc any.  bias f32 [N] or NULL.
+ * An operand is its code times its scale as an fp32 value; one of 2^128 or more may count as infinite, one under 2^-133 as zero.
  * workspace: merlot_gemm_f8_blocks_workspace_bytes(M, N, K) bytes, 16-byte aligned, any content (partial products of reductions that are split over workgroups and
  * folded in a fixed order; may be NULL where that is 0). */
 int64_t merlot_gemm_f8_blocks_workspace_bytes(int64_t M, int64_t N, int64_t K);

@@ -137,7 +137,7 @@ extern "C" int merlot_quantize_blocks(const void* x, int64_t ldx, int x_f32, int
     MERLOT_CHECK(fmt == 0 || fmt == 1, MERLOT_EDTYPE, "merlot_quantize_blocks: fmt must be 0 (e4m3) or 1 (e5m2)");
     MERLOT_CHECK(tile == 1 || tile == 128, MERLOT_ESHAPE, "merlot_quantize_blocks: tile must be 1 or 128");
     const int64_t tr = (R + 127) / 128, tc = (C + 127) / 128;
-    MERLOT_CHECK(tr * tc < ((int64_t)1 << 31), MERLOT_ESHAPE, "merlot_quantize_blocks: too many tiles");
+    MERLOT_CHECK(tr * tc < ((int64_t)1 << 24), MERLOT_ESHAPE, "merlot_quantize_blocks: too many tiles");
     MERLOT_CHECK(!q || (ldq >= tc * 128 && ldq % 16 == 0 && lds >= tc), MERLOT_ESHAPE, "merlot_quantize_blocks: the row-wise copy has ceil(C / 128) * 128 columns and a scale per 128");
     MERLOT_CHECK(!qt || (ldqt >= tr * 128 && ldqt % 16 == 0 && ldst >= tr), MERLOT_ESHAPE, "merlot_quantize_blocks: the transposed copy has ceil(R / 128) * 128 columns and a scale per 128");
     MERLOT_CHECK((((uintptr_t)q | (uintptr_t)qt) & 15) == 0, MERLOT_EALIGN, "merlot_quantize_blocks: the copies must be 16-byte aligned");

@@ -135,6 +135,69 @@ def test_product_against_64_bits(M, N, K, fa):
         assert torch.equal(got, ops.gemm_f8_blocks(a, sa, b, sb, out_dtype=dt))
 
 
+def _whole_on_device(rows, K, fmt, seed):
+    """_operand(whole=True) made on the device, values in fp32"""
+    g = torch.Generator(device='cuda').manual_seed(seed)
+    v = torch.randint(-8, 9, (rows, K), generator=g, device='cuda').float()
+    e = torch.randint(0, 3, (rows, K // 128), generator=g, device='cuda')
+    wide = torch.full((rows, (K // 128 + 3) // 4 * 4), 255, dtype=torch.uint8, device='cuda')
+    wide[:, :K // 128] = (127 + e).to(torch.uint8)
+    return v.to(ref.FORMATS[fmt][0]), wide[:, :K // 128], v * (1 << e).float().repeat_interleave(128, 1)
+
+
+# (M, N, K) by the kernel they take.  256 x 256 tiles (bf16 outputs): whole tiles, ragged ones, rows of C that are no whole sectors (N = 4300: K = 2 048 on), more than sixteen
+# blocks, more tiles than workgroups; 128 x 256 tiles: short K, fp32, odd N; split reductions with either width
+@pytest.mark.parametrize('M,N,K', [(4096, 4096, 512), (8200, 2080, 640), (4100, 4384, 2304), (4200, 4300, 2176), (20000, 1120, 768), (33000, 512, 256), (33000, 500, 384), (2304, 768, 6272),
+                                   (300, 200, 9216), (16500, 1028, 128)])
+@pytest.mark.parametrize('fa', [0, 1])
+def test_large_products_of_whole_numbers_are_exact(M, N, K, fa):
+    """|sum| <= 64 * 16 * K < 2^24: exact in fp32 in any order, in every kernel; the fp32 reference product is exact for the same reason"""
+    ops = _ops()
+    a, sa, va = _whole_on_device(M, K, fa, 5)
+    b, sb, vb = _whole_on_device(N, K, 0, 6)
+    bias = torch.randint(-50, 50, (N,), device='cuda').float()
+    want = va @ vb.t() + bias
+    assert float(want.abs().max()) < 2 ** 24
+    for dt in (torch.bfloat16, torch.float32):
+        buf = torch.full((M + 1, N), 7.0, device='cuda', dtype=dt)
+        got = ops.gemm_f8_blocks(a, sa, b, sb, bias=bias, out=buf[:M])
+        assert torch.equal(got, want.to(dt)), dt
+        assert bool((buf[M] == 7).all())
+    c = torch.randint(-9, 9, (M, N), device='cuda').float()
+    assert torch.equal(ops.gemm_f8_blocks(a, sa, b, sb, out=c.clone(), accumulate=True), c + (want - bias))
+
+
+@pytest.mark.parametrize('N', [3, 300, 5000])
+@pytest.mark.parametrize('M', [5, 70, 600])
+def test_least_and_largest_scales(M, N):
+    """byte 0 (2^-127) against byte 251 (2^124): whole numbers again, through operands under the normal range.  An operand is its code times its scale in fp32: 8 * 2^124 = 2^127 is the
+    largest power that is finite there, so that byte 254 would make every |code| > 1 infinite (8 * 2^127 = 2^130)"""
+    ops = _ops()
+    a, sa, _ = _whole_on_device(M, 256, 0, 1)
+    b, sb, _ = _whole_on_device(N, 256, 0, 2)
+    sa.fill_(0); sb.fill_(251)
+    want = (a.float() @ b.float().t()) / 8
+    assert torch.equal(ops.gemm_f8_blocks(a, sa, b, sb, out_dtype=torch.float32), want)
+    assert torch.equal(ops.gemm_f8_blocks(a, sa, b, sb), want.bfloat16())
+    assert torch.equal(ops.gemm_f8_blocks(b, sb, a, sa, out_dtype=torch.float32), want.t())
+
+
+def test_large_product_against_64_bits():
+    """256 x 256 tiles on real operands: the 8-bit matrix instruction's own tolerance"""
+    ops = _ops()
+    for M, N, K in ((5000, 3520, 768), (4352, 4096, 2432)):
+        g = torch.Generator(device='cuda').manual_seed(K)
+        x, w = torch.randn(M, K, generator=g, device='cuda').bfloat16(), torch.randn(N, K, generator=g, device='cuda').bfloat16()
+        a, sa = ops.quantize_blocks(x)
+        b, sb = ops.quantize_blocks(w, tile=128)
+        va, vb = ref.values(a, sa).cuda(), ref.values(b, sb).cuda()
+        want, mag = va @ vb.t().contiguous(), va.abs() @ vb.abs().t().contiguous()
+        got = ops.gemm_f8_blocks(a, sa, b, sb)
+        assert bool(((got.double() - want).abs() <= ((K + 64) * 2.0 ** -23 + 7 * 2.0 ** -13) * mag * (1 + 2.0 ** -8) + 2.0 ** -8 * want.abs()).all())
+        assert float((got.double() - want).norm() / want.norm()) < 2.0 ** -8
+        assert torch.equal(got, ops.gemm_f8_blocks(a, sa, b, sb))
+
+
 def test_product_with_extreme_scales_and_nan_blocks():
     ops = _ops()
     a, sa, _ = _operand(70, 256, 0, 1, whole=True)
@@ -289,6 +352,45 @@ def test_norm_product_and_clip_together():
     for got, want in ((z, zr), (xg.grad, dxr), (norm.ggamma, dg * 0.5 / nr), (lin.gw, gw * 0.5 / nr), (lin.gb, gb * 0.5 / nr), (n, torch.tensor(nr).double())):
         assert float((got.detach().double().cpu() - want).norm()) <= (2.0 ** -3 * 0.1 + 3 * 2.0 ** -8) * float(want.norm())
     assert torch.equal(h.cpu(), hr)
+
+
+def test_two_streams_at_once_and_another_current_device(monkeypatch):
+    """the same calls in flight on two streams: no workspace is shared; and tensors of a device that is not the current one are refused"""
+    ops = _ops()
+    ins = []
+    for k in range(2):
+        x, w = torch.randn(300, 5000 + k, device='cuda').bfloat16(), torch.randn(400, 5000 + k, device='cuda').bfloat16()
+        grads = [torch.randn(5000, device='cuda') for _ in range(130)]
+        ins.append((x, w, torch.rand(5000 + k, device='cuda'), grads))
+
+    def work(x, w, gamma, grads):
+        outs = [torch.empty_like(t) for t in grads]
+        y, _, rstd, y8, s8 = ops.rms_norm_fwd(x, gamma, q8=True)
+        b8, sb = ops.quantize_blocks(w, tile=128)
+        dg = torch.zeros_like(gamma)
+        dx = ops.rms_norm_bwd(y, x, rstd, gamma, dg)
+        return [ops.gemm_f8_blocks(y8, s8, b8, sb, out_dtype=torch.float32), dx, dg, ops.clip_by_global_norm(grads, 0.5, out=outs)] + outs
+    want = [[t.clone() for t in work(*i)] for i in ins]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    got = [None, None]
+    for _ in range(5):
+        for k, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[k] = work(*ins[k])
+    torch.cuda.synchronize()
+    for a, b in zip(got, want):
+        for u, v in zip(a, b):
+            assert torch.equal(u, v)
+    x, w, gamma, grads = ins[0]
+    kept = ops.TensorList(grads)
+    q, s = ops.quantize_blocks(x)
+    monkeypatch.setattr(torch.cuda, 'current_device', lambda: 1)
+    for fn in (lambda: ops.rms_norm_fwd(x, gamma), lambda: ops.quantize_blocks(x), lambda: ops.gemm_f8_blocks(q, s, q, s), lambda: ops.global_norm(kept)):
+        with pytest.raises(ValueError, match='current device'):
+            fn()
 
 
 def test_captured_step_replays_on_new_inputs_and_streams():
