@@ -1110,6 +1110,7 @@ __device__ __forceinline__ void weight_std_bwd_body(const float* __restrict__ dk
     float s1 = 0.f, s2 = 0.f;
 #pragma unroll 8
     for (int r = kl; r < K; r += WS_K) {
+#pragma clang fp contract(off)                           // (the products are rounded whatever instructions the compiler may use: the same bits in every build)
         const float d = dkt[(int64_t)cc * ld + r];
         s1 += d;
         s2 += d * khat[(int64_t)r * Co + cc];

@@ -87,15 +87,27 @@ __global__ __launch_bounds__(256) void ln_fwd_kernel(const TX* __restrict__ x, c
 #pragma unroll
         for (int i = 0; i < NS; ++i) nxt[i] = load_raw<TX>(x + (row + stride) * H + i * 256 + lane * 4);
     }
-    const float mean = wave_sum(s) * (1.0f / H);
-    float ss = 0.f;
+    // which products are fused into sums is written out, here and in the backward: left to the compiler it depends on the instructions it may use, and with it the last
+    // bits of every activation (forward: the squares of the last slab and of element 1 are rounded, the others not; backward: dy * gamma is rounded but in the first slab's dx)
+    const float sum = wave_sum(s);
+    float ss = 0.f, mean, first = 0.f;
 #pragma unroll
-    for (int i = 0; i < NS; ++i)
+    for (int i = 0; i + 1 < NS; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const float d = v[i][e] - mean;
+            const float d = fmaf(sum, -1.0f / H, v[i][e]);
+            if (i == 0 && e == 0) first = d;
+            else ss = i == 0 && e == 1 ? fmaf(first, first, d * d) : fmaf(d, d, ss);
+        }
+    {
+#pragma clang fp contract(off)
+        mean = sum * (1.0f / H);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float d = v[NS - 1][e] - mean;
             ss += d * d;
         }
+    }
     const float var = wave_sum(ss) * (1.0f / H);
     const float rstd = rsqrtf(var + eps);
     float amax = 0.f;
@@ -219,21 +231,34 @@ __global__ __launch_bounds__(256) void ln_bwd_kernel(const TDY* __restrict__ dy,
             float (&xv)[4] = xvv[i];
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
+#pragma clang fp contract(off)
                 xh[i][e] = (xv[e] - mu) * rs;
                 const float gd = dyv[i][e] * g[i][e];
                 c1 += gd;
                 c2 += gd * xh[i][e];
-                dg[i][e] += dyv[i][e] * xh[i][e];
+                dg[i][e] = fmaf(dyv[i][e], xh[i][e], dg[i][e]);
                 db[i][e] += dyv[i][e];
             }
         }
-        c1 = wave_sum(c1) * (1.0f / H);
-        c2 = wave_sum(c2) * (1.0f / H);
+        {
+#pragma clang fp contract(off)
+            c1 = wave_sum(c1) * (1.0f / H);
+            c2 = wave_sum(c2) * (1.0f / H);
+        }
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             float o[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = rs * (dyv[i][e] * g[i][e] - c1 - xh[i][e] * c2);
+            for (int e = 0; e < 4; ++e) {
+                float t;
+                if (i == 0) {
+                    t = fmaf(dyv[i][e], g[i][e], -c1);
+                } else {
+#pragma clang fp contract(off)
+                    t = dyv[i][e] * g[i][e] - c1;
+                }
+                o[e] = rs * fmaf(-c2, xh[i][e], t);
+            }
             if (dres) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) o[e] += rv[i][e];
