@@ -587,39 +587,26 @@ class RMSNormFn(torch.autograd.Function):
 
 def rms_norm(x, norm, residual=None, eps=1e-6):
     """root-mean-square norm over the last dimension with the gain of `norm` (a ParamStore.ln handle: gamma, and ggamma, which the backward ACCUMULATES into).
-    x bf16 or f32 [..., H]; with a residual of the same type and shape: -> (y, h = x + residual), both differentiable."""
+    x bf16 or f32 [..., H]; with a residual of the same type and shape: -> (y, h = x + residual), both differentiable.  The backward runs where x or the residual
+    requires a gradient."""
     return RMSNormFn.apply(x, residual, norm, eps)
-
-
-def _w8_blocks(lin):
-    """the 8-bit copies of a Linear's bf16 working weight, both orientations in 128 x 128 tiles: made once per version of the working copies and stream (they change
-    at the optimizer step only).  A captured launch makes its own: a replay has to see the weights of ITS time.  A new version gets new tensors, so a backward
-    that is still to come keeps the copies its forward used."""
-    store = lin._store
-    if store is None or torch.cuda.is_current_stream_capturing():
-        return ops.quantize_blocks(lin.wb, tile=128, transpose=True)
-    cache = store.__dict__.setdefault('_w8_blocks', {})
-    key = (lin.name, torch.cuda.current_stream().cuda_stream)
-    ent = cache.get(key)
-    if ent is None or ent[0] != store.version:
-        ent = cache[key] = (store.version, ops.quantize_blocks(lin.wb, tile=128, transpose=True))
-    return ent[1]
 
 
 class LinearF8BlocksFn(torch.autograd.Function):
     """y = x W^T + b with all three products of the layer on 8-bit blocks (ops.gemm_f8_blocks).  x is quantised once, row-wise for this product and transposed for
-    the weight gradient: what waits for the backward is the one-byte transposed copy, not x."""
+    the weight gradient, the weight once in both orientations (every forward anew: a few microseconds, and never a copy of older weights): what waits for the
+    backward are the one-byte transposed copies, not x."""
 
     @staticmethod
     def forward(ctx, x, lin, grad_fmt):
         if lin.gb is not None and lin.w.shape[0] % 4 != 0:
             raise ValueError("linear_f8_blocks: a Linear with a bias needs an output width that is a multiple of 4 (the bias gradient's column sums)")
         x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-        w8, sw, wt8, swt = _w8_blocks(lin)
         if ctx.needs_input_grad[0]:
+            w8, sw, wt8, swt = ops.quantize_blocks(lin.wb, tile=128, transpose=True)
             x8, sx, xt8, sxt = ops.quantize_blocks(x2, transpose=True)
-        else:
-            (x8, sx), xt8, sxt = ops.quantize_blocks(x2), None, None
+        else:                                            # no graph: nothing waits for a backward
+            (w8, sw), (x8, sx), xt8, sxt, wt8, swt = ops.quantize_blocks(lin.wb, tile=128), ops.quantize_blocks(x2), None, None, None, None
         ctx.lin, ctx.grad_fmt, ctx.shape, ctx.dtype = lin, grad_fmt, x.shape, x.dtype
         ctx.save_for_backward(xt8, sxt, wt8, swt)
         return ops.gemm_f8_blocks(x8, sx, w8, sw, bias=lin.b).view(*x.shape[:-1], lin.w.shape[0])
@@ -640,7 +627,8 @@ class LinearF8BlocksFn(torch.autograd.Function):
 
 def linear_f8_blocks(x, lin, grad_fmt=ops.F8_E4M3):
     """x [..., in] (bf16 or f32) -> bf16 [..., out]; weight and bias gradients are ACCUMULATED into the Linear's gradient views.  Operands are e4m3 with a scale per
-    128 values along each product's reduction (activations) or per 128 x 128 tile (weights); grad_fmt: the format of dy."""
+    128 values along each product's reduction (activations) or per 128 x 128 tile (weights); grad_fmt: the format of dy.  As with every layer here whose parameters live
+    in a store, the backward runs where x requires a gradient."""
     return LinearF8BlocksFn.apply(x, lin, grad_fmt)
 
 

@@ -302,6 +302,10 @@ def test_linear_of_a_store_follows_its_weights():
     with torch.no_grad():
         y2 = layers.linear_f8_blocks(x, lin)
     assert torch.equal(y1, -y2) or float((y1 + y2).abs().max()) <= 2 * float(lin.b.abs().max())
+    lin.w.mul_(-1.0)
+    st.refresh(force=True)                               # the same version, other weights
+    with torch.no_grad():
+        assert torch.equal(layers.linear_f8_blocks(x, lin), y1)
     dy = torch.randn_like(y1)
     y1.backward(dy)
     d8, sd = ops.quantize_blocks(dy.view(10, -1))
