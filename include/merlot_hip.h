@@ -572,7 +572,7 @@ int merlot_quantize_blocks(const void* x, int64_t ldx, int x_f32, int64_t R, int
                            int64_t lds, void* qt, int64_t ldqt, uint8_t* st, int64_t ldst, merlot_stream_t stream);
 /* C[M,N] (+)= sum over blocks b of 128 of 2^(scale_a[m,b] - 127 + scale_b[n,b] - 127) * (A8[m,b] . B8[n,b]) (+ bias[n]): operands as merlot_quantize_blocks
  * writes them, A8 e4m3 (fmt_a 0) or e5m2 (1), B8 e4m3; K % 128 == 0, M and N any; operand rows 16-byte, scale rows 4-byte aligned (leading dimensions too) and
- * read in whole words of 4 bytes.  fp32 accumulators; an f32 C is good to fp32 (the codes go through the bf16 matrix instruction, exactly), a bf16 C comes from the
+ * read in whole words of 4 bytes; lda, ldb, ld_scale_* under 2^22, M and N under 2^31 - 256.  fp32 accumulators; an f32 C is good to fp32 (the codes go through the bf16 matrix instruction, exactly), a bf16 C comes from the
  * 8-bit instruction, which keeps 13 bits below the largest of each eight products.  C bf16 or f32 (out_f32; accumulate adds into C before the one rounding), ldc any.  bias f32 [N] or NULL.
  * An operand is its code times its scale as an fp32 value; one of 2^128 or more may count as infinite, one under 2^-133 as zero.
  * workspace: merlot_gemm_f8_blocks_workspace_bytes(M, N, K) bytes, 16-byte aligned, any content (partial products of reductions that are split over workgroups and

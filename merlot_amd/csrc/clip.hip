@@ -183,6 +183,7 @@ extern "C" int merlot_clip_by_global_norm(const int64_t* in, const int64_t* out,
     MERLOT_CHECK(clip >= 0.f && clip <= 3.402823466e38f, MERLOT_ESHAPE, "merlot_clip_by_global_norm: clip must be 0 (the norm alone) or positive and finite");
     MERLOT_CHECK(clip == 0.f || out, MERLOT_ESHAPE, "merlot_clip_by_global_norm: null operand");
     MERLOT_CHECK(workspace && workspace_bytes >= merlot_clip_workspace_bytes(n), MERLOT_ESHAPE, "merlot_clip_by_global_norm: workspace too small");
+    MERLOT_CHECK(((uintptr_t)workspace & 7) == 0, MERLOT_EALIGN, "merlot_clip_by_global_norm: workspace must be 8-byte aligned");
     for (int64_t i = 0; i < n; ++i) {
         MERLOT_CHECK(numel[i] >= 0 && numel[i] < ((int64_t)1 << 40), MERLOT_ESHAPE, "merlot_clip_by_global_norm: tensor %lld has a bad size", (long long)i);
         MERLOT_CHECK(types[i] < 4, MERLOT_EDTYPE, "merlot_clip_by_global_norm: tensor %lld has a bad type", (long long)i);

@@ -479,6 +479,8 @@ __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p)
         if (!last) {
             ask_scales(next_tile, 0);
             ask_bias(next_tile);
+        } else {
+            wait_step<0>();                              // the fetches ahead (zeros, from buffers without a byte) have left the LDS before the workgroup does
         }
         // ---- epilogue: units of 32 rows x 64 columns through the wave's slab (16-byte chunk c of row r at c ^ (r & 7)).  Unit u + 1 is rounded while unit u's writes and reads
         // travel, and unit u is stored behind that: nothing waits for the slab.

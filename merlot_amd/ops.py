@@ -1033,7 +1033,7 @@ def _scale_ld(s, rows, nb, name):
 
 def gemm_f8_blocks(a8, a_scale, b8, b_scale, *, bias=None, out=None, out_dtype=BF16, accumulate=False):
     """C[M,N] (+)= a8[M,K] @ b8[N,K]^T (+ bias) on 8-bit operands with a scale per row and block of 128, as quantize_blocks / rms_norm_fwd(q8=True) make them: a8 e4m3
-    or e5m2, b8 e4m3, K a multiple of 128; M, N any.  fp32 accumulation; C bf16 or f32 (out / out_dtype), accumulate (f32 out only) adds into out."""
+    or e5m2, b8 e4m3, K a multiple of 128, row strides under 2^22; M, N any.  fp32 accumulation; C bf16 or f32 (out / out_dtype), accumulate (f32 out only) adds into out."""
     fa = 1 if a8.dtype == torch.float8_e5m2 else 0
     _operands((a8, _F8_DTYPES[fa], 'a8'), (b8, FP8, 'b8'), (a_scale, torch.uint8, 'a_scale'), (b_scale, torch.uint8, 'b_scale'), (bias, F32, 'bias'))
     if a8.dim() != 2 or b8.dim() != 2 or a8.shape[1] != b8.shape[1] or a8.shape[1] == 0 or a8.shape[1] % 128 != 0:

@@ -98,7 +98,8 @@ class AdamOptimizer(object):
         for s_, e_ in self.frozen:
             g[s_:e_].zero_()
         if g.is_cuda:                                         # two launches over the arena (2e8 addends: summed in fp64)
-            return ops.clip_by_global_norm([g], self.clip_norm) if self.clip_norm > 0.0 else ops.global_norm([g])
+            with torch.cuda.device(g.device):
+                return ops.clip_by_global_norm([g], self.clip_norm) if self.clip_norm > 0.0 else ops.global_norm([g])
         norm = torch.linalg.vector_norm(g, dtype=torch.float64).float()   # an arena in host memory (no device kernels there)
         if self.clip_norm > 0.0:
             g.mul_(self.clip_norm / torch.clamp(norm, min=self.clip_norm))
