@@ -9,6 +9,7 @@
 //   * fp32 outputs (a weight gradient added to others, logits): that would be the largest error there is.  A code times a power of two is a bf16 value, so the
 //     fragments are converted exactly (v_cvt_scalef32_pk_bf16_*, the scale included) and go through v_mfma_f32_32x32x16_bf16, whose sums are good to fp32.  Half the
 //     matrix rate, still 8-bit traffic.
+#include <utility>
 #include "blocks8.h"
 
 namespace {
@@ -18,13 +19,16 @@ struct BlocksArgs {
     int64_t lda, ldb, ldsa, ldsb;
     void* C; int64_t ldc;
     const float* bias;
-    float* part;                             // split reductions: [splits][M][N] partial products
+    float* part;                             // split reductions: [splits][M][part_ld(N)] partial products
     int64_t M, N;
-    int nk, nk_split;                        // blocks of 128 in all, per split
+    int nk, nk_split, splits;                // blocks of 128 in all, per split
     int ntm, ntn;
     int accumulate;
     unsigned band_magic;                     // 2^32 / (4 ntn): blocks_wide_kernel
 };
+
+// rows of partial products start at multiples of 64 bytes, whatever N
+__host__ __device__ __forceinline__ int64_t part_ld(int64_t N) { return (N + 15) & ~(int64_t)15; }
 
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t rows_rsrc(const uint8_t* p, int64_t row0, int64_t rows, int64_t ld, int64_t width) {
     // the rows of one tile as a buffer of their own: offsets stay small however large the operand is, and rows past its end read as zeros
@@ -253,8 +257,8 @@ __global__ __launch_bounds__(256, 2) void blocks_gemm_kernel(const BlocksArgs p)
     constexpr int COLS = BN / 2, LDR = COLS * (int)sizeof(T) + 16, E = 16 / (int)sizeof(T), LPR = COLS / E;      // slab row in bytes; 16-byte groups per row
     static_assert(4 * 32 * LDR <= 3 * STEP, "slabs");
     uint8_t* const slab = lds + wave * 32 * LDR;
-    T* const C = OUT == 2 ? (T*)p.part + (int64_t)blockIdx.y * p.M * p.N : (T*)p.C;
-    const int64_t ldc = OUT == 2 ? p.N : p.ldc, n = n0 + wn * COLS + (lane % LPR) * E;
+    const int64_t ldc = OUT == 2 ? part_ld(p.N) : p.ldc, n = n0 + wn * COLS + (lane % LPR) * E;
+    T* const C = OUT == 2 ? (T*)p.part + (int64_t)blockIdx.y * p.M * ldc : (T*)p.C;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -282,25 +286,34 @@ __global__ __launch_bounds__(256, 2) void blocks_gemm_kernel(const BlocksArgs p)
 // Large outputs: 256 x 256 tiles, four waves of 128 x 128 -- ONE per SIMD, 256 accumulators each --, K-tiles of 128 (whole 128-byte lines per row, where 64-byte steps
 // ask the L2 twice per line), two K-tile buffers.  A wave's next fragments are read, and the next K-tile is fetched, between its own matrix instructions; the one barrier
 // per K-tile stands where the buffer's last reads have returned.  Persistent: workgroups walk the tiles of their XCD's band, the fetch stream runs on across tile ends, and
-// a tile's stores drain while the next one multiplies.
+// a tile's stores drain while the next one multiplies.  fp32 outputs convert two fragment slices between every four matrix instructions: with 128 x 128 per wave that is two
+// conversions a matrix instruction, with 64 x 128 three (8192^3: 787 us = 1.4 PFLOP/s, the rate of a large bf16 product, against 870).
 constexpr int WIDE_BUF = 65536, WIDE_SCALES = 2 * WIDE_BUF, WIDE_BIAS = WIDE_SCALES + 512 * SCALE_BLOCKS, WIDE_SLAB = WIDE_BIAS + 2048;
 constexpr int WIDE_LDS = WIDE_SLAB + 4 * 4096;           // two K-tiles, 16 blocks' scale bytes of 512 rows, two tiles' bias, a slab of 32 rows x 128 bytes per wave
 
+template <typename F, int... U>
+__device__ __forceinline__ void units(F& f, std::integer_sequence<int, U...>) { (f(std::integral_constant<int, U>{}), ...); }
+
 // LINES: rows of C start at multiples of 64 bytes -- stored past the caches (a template: two branches with the same store would be merged into an ordinary one)
-template <int FA, bool LINES>
+// OUT: 0 bf16, 1 fp32, 2 fp32 partial products of a split reduction; fp32 through bf16 fragments (the work items are (split, tile), split by split)
+template <int FA, bool LINES, int OUT>
 __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p) {
 #ifdef __HIP_DEVICE_COMPILE__
+    constexpr bool EXACT = OUT != 0;
+    typedef typename std::conditional<EXACT, float, bf16>::type T;
     extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hi = lane >> 5, l31 = lane & 31, wm = wave >> 1, wn = wave & 1;
-    const int ntiles = p.ntm * p.ntn, nwg = gridDim.x, nk = p.nk;
+    const int ntiles = p.ntm * p.ntn, nwg = gridDim.x;
     // XCD x's band of tiles, and this workgroup's walk through it
-    const int xcd = (int)blockIdx.x & 7, q8 = ntiles >> 3, r8 = ntiles & 7;
+    const int items = OUT == 2 ? ntiles * p.splits : ntiles;
+    const int xcd = (int)blockIdx.x & 7, q8 = items >> 3, r8 = items & 7;
     const int band = xcd < r8 ? xcd * (q8 + 1) : r8 * (q8 + 1) + (xcd - r8) * q8, band_end = band + q8 + (xcd < r8 ? 1 : 0);
     const int stride = (nwg >> 3) + (xcd < (nwg & 7) ? 1 : 0);
     int tile = band + ((int)blockIdx.x >> 3);
     if (tile >= band_end) return;
-    auto place = [&](int id, int& m0, int& n0) {         // bands of four tile rows, column by column (an XCD's 32 CUs: about 4 x 8 tiles)
+    auto place = [&](int id, int& m0, int& n0) __attribute__((always_inline)) {         // bands of four tile rows, column by column (an XCD's 32 CUs: about 4 x 8 tiles)
+        if constexpr (OUT == 2) id = (int)((unsigned)id % (unsigned)ntiles);
         const unsigned d = 4u * (unsigned)p.ntn;
         unsigned b = __umulhi((unsigned)id, p.band_magic), in = (unsigned)id - b * d;     // floor(2^32 / d): the quotient or one less
         if (in >= d) { ++b; in -= d; }
@@ -309,7 +322,9 @@ __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p)
         m0 = (int)(b * 4u + in - c * high) * 256;
         n0 = (int)c * 256;
     };
-    const int64_t K = (int64_t)nk * 128;
+    auto first_of = [&](int id) __attribute__((always_inline)) -> int { return OUT == 2 ? (int)((unsigned)id / (unsigned)ntiles) * p.nk_split : 0; };
+    auto count_of = [&](int first) __attribute__((always_inline)) -> int { return OUT == 2 ? min(p.nk_split, p.nk - first) : p.nk; };
+    const int64_t K = (int64_t)p.nk * 128;
     // ---- fetch stream: 32 pieces of 8 rows x 128 bytes per operand and K-tile, 8 + 8 per wave.  Image: row r at r * 128, its 16-byte chunk c at c ^ ((r >> 1) & 7)
     unsigned offa[8], offb[8];
 #pragma unroll
@@ -320,18 +335,19 @@ __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p)
         offb[i] = (unsigned)(row * p.ldb) + ch;
     }
     __amdgpu_buffer_rsrc_t ra, rb;
-    int s_tile = tile, s_kt = 0;
-    auto stream_to = [&](int id) {
+    int s_tile = tile, s_kt = 0, s_end = p.nk;
+    auto stream_to = [&](int id) __attribute__((always_inline)) {
         int m = 0, n = 0;
+        s_kt = first_of(id);
+        s_end = s_kt + count_of(s_kt);
         if (id < band_end) place(id, m, n);              // (behind the last tile: buffers without a byte -- the two K-tiles fetched ahead touch no memory)
         ra = rows_rsrc(p.A, m, id < band_end ? min((int64_t)256, p.M - m) : 0, p.lda, K);
         rb = rows_rsrc(p.B, n, id < band_end ? min((int64_t)256, p.N - n) : 0, p.ldb, K);
     };
     auto fetch_a = [&](int i, int buf) { __builtin_amdgcn_raw_ptr_buffer_load_lds(ra, LDS_PTR(lds + buf + (wave * 8 + i) * 1024), 16, offa[i], s_kt * 128, 0, 0); };
     auto fetch_b = [&](int i, int buf) { __builtin_amdgcn_raw_ptr_buffer_load_lds(rb, LDS_PTR(lds + buf + 32768 + (wave * 8 + i) * 1024), 16, offb[i], s_kt * 128, 0, 0); };
-    auto advance = [&]() {                               // to the stream's next K-tile
-        if (++s_kt == nk) {
-            s_kt = 0;
+    auto advance = [&]() __attribute__((always_inline)) {                               // to the stream's next K-tile
+        if (++s_kt == s_end) {
             s_tile += stride;
             stream_to(s_tile);
         }
@@ -339,9 +355,10 @@ __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p)
     // ---- scale words (16 blocks of 512 rows: eight words per thread) and bias, through registers into LDS
     int sw[8];
     float bias_reg;
-    auto ask_scales = [&](int id, int kb) {
+    auto ask_scales = [&](int id, int kb) {              // kb: within the item
         int m, n;
         place(id, m, n);
+        kb += first_of(id);
         const int64_t width = (p.nk + 3) & ~3;
         const __amdgpu_buffer_rsrc_t rsa = rows_rsrc(p.sa, m, min((int64_t)256, p.M - m), p.ldsa, width), rsb = rows_rsrc(p.sb, n, min((int64_t)256, p.N - n), p.ldsb, width);
 #pragma unroll
@@ -383,16 +400,37 @@ __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p)
     // chunk f (0 ... 15) of the fragments of half H in the order the products ask for them: B 0, A 0, A 1, A 2, A 3, B 1, B 2, B 3
     auto read_chunk = [&](auto hc, int f, unsigned base) __attribute__((always_inline)) {
         constexpr int H = decltype(hc)::value;
-        const int k = f >> 1, part = f & 1;
+        // (fp32: the first halves of all fragments, which are converted first, then the others)
+        const int k = EXACT ? f & 7 : f >> 1, part = EXACT ? f >> 3 : f & 1;
         if (k == 0 || k >= 5) { const int j = k == 0 ? 0 : k - 4; fb[H][j][part] = chunk(base + frb + j * 4096, H, part); }
         else fa[H][k - 1][part] = chunk(base + fra + (k - 1) * 4096, H, part);
+    };
+    // fp32: slice q (16 of the half K-tile's 64, eight per half wave) of the fragments as bf16, the scale included; the next slice is converted between the products
+    bf16x8 wa[2][4], wb[2][4];                           // [parity of the slice]
+    float va[4], vb[4];                                  // the block's scales
+    auto scale_floats = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            va[i] = scale_value(xa[i] & 255);
+            vb[i] = scale_value(xb[i] & 255);
+        }
+    };
+    auto convert = [&](auto hc, int q, int f) __attribute__((always_inline)) {       // f: 0 ... 3 rows of A, 4 ... 7 of B
+        constexpr int H = decltype(hc)::value;
+        if (f < 4) wa[q & 1][f] = widen<FA>(fa[H][f][q >> 1][2 * (q & 1)], fa[H][f][q >> 1][2 * (q & 1) + 1], va[f]);
+        else wb[q & 1][f - 4] = widen<0>(fb[H][f - 4][q >> 1][2 * (q & 1)], fb[H][f - 4][q >> 1][2 * (q & 1) + 1], vb[f - 4]);
     };
     // one half K-tile: the products with the fragments of half P; between them the other half's fragments are read from the buffer at `next`, and with FETCH the stream's
     // K-tile is fetched into the one at `into`
     auto half = [&](auto pc, auto firstc, auto fetchc, unsigned next, int into) __attribute__((always_inline)) {
         constexpr int P = decltype(pc)::value;
         constexpr bool FIRST = decltype(firstc)::value, FETCH = decltype(fetchc)::value;
-        // sixteen slots of one matrix instruction (64 cycles): one read and one fetch in half 1; in half 0 two reads in each of the first eight, so that they have returned
+        if constexpr (EXACT && P == 0) {
+            scale_floats();
+#pragma unroll
+            for (int f = 0; f < 8; ++f) convert(pc, 0, f);
+        }
+        // sixteen slots of one matrix instruction (64 cycles; fp32: 128): one read and one fetch in half 1; in half 0 two reads in each of the first eight, so that they have returned
         // where the barrier behind the half asks for it
 #pragma unroll
         for (int k = 0; k < 16; ++k) {
@@ -407,7 +445,22 @@ __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p)
                 if (k & 1) fetch_b(k >> 1, into);
                 else fetch_a(k >> 1, into);
             }
-            acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(whole(fb[P][j]), whole(fa[P][i]), FIRST ? zero : acc[i][j], 0, FA, 0, xb[j], 0, xa[i]);
+            if constexpr (!EXACT) {
+                acc[i][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(whole(fb[P][j]), whole(fa[P][i]), FIRST ? zero : acc[i][j], 0, FA, 0, xb[j], 0, xa[i]);
+            } else {                                     // a slot: column j of slice q = k / 4, four matrix instructions of 32 cycles
+                const int q = k >> 2, c = k & 3;
+                // the next slice's fragments, two a slot; behind half 0 those of half 1 (half 0's own first slice waits for its block's scales)
+                if (q < 3) {
+                    convert(pc, q + 1, 2 * c);
+                    convert(pc, q + 1, 2 * c + 1);
+                } else if (P == 0) {
+                    convert(std::integral_constant<int, 1>{}, 0, 2 * c);
+                    convert(std::integral_constant<int, 1>{}, 0, 2 * c + 1);
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    acc[r][c] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(wb[q & 1][c], wa[q & 1][r], FIRST && q == 0 ? zero : acc[r][c], 0, 0, 0);
+            }
             __builtin_amdgcn_sched_barrier(0);
         }
 #pragma unroll
@@ -447,6 +500,7 @@ __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p)
         place(tile, m0, n0);
         const int next_tile = tile + stride;
         const bool last = next_tile >= band_end;
+        const int kb0 = first_of(tile), nk = count_of(kb0);          // the item's blocks
         read_scales(0);
         auto ktile = [&](int kt, auto firstc) __attribute__((always_inline)) {
             half(c0_t{}, firstc, no_t{}, buf, 0);
@@ -482,59 +536,69 @@ __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p)
         } else {
             wait_step<0>();                              // the fetches ahead (zeros, from buffers without a byte) have left the LDS before the workgroup does
         }
-        // ---- epilogue: units of 32 rows x 64 columns through the wave's slab (16-byte chunk c of row r at c ^ (r & 7)).  Unit u + 1 is rounded while unit u's writes and reads
+        // ---- epilogue: units of 32 rows x 64 columns (fp32: 32) through the wave's slab (16-byte chunk c of row r at c ^ (r & 7)).  Unit u + 1 is rounded while unit u's writes and reads
         // travel, and unit u is stored behind that: nothing waits for the slab.
         uint8_t* const slab = lds + WIDE_SLAB + wave * 4096;
         int el = lane;                                   // the epilogue's addresses are made here, tile by tile: hoisted out of the tile loop they would fill the registers
         asm volatile("" : "+v"(el));
         const int e31 = el & 31, eh = el >> 5;
         const bool inside = m0 + 256 <= p.M && n0 + 256 <= p.N;
-        const int64_t row0 = m0 + wm * 128 + (el >> 3), col0 = n0 + wn * 128 + (el & 7) * 8;
+        constexpr int E = 16 / (int)sizeof(T), UC = 8 * E;           // values per lane, columns per unit
+        const int64_t row0 = m0 + wm * 128 + (el >> 3), col0 = n0 + wn * 128 + (el & 7) * E;
         const int m_left = (int)max((int64_t)-1, min(p.M - row0, (int64_t)256)), n_left = (int)max((int64_t)-1, min(p.N - col0, (int64_t)256));
-        bf16* out = (bf16*)p.C + row0 * p.ldc + col0;    // this lane's piece of the slab's rows 0 ... 7
-        bf16x4 o[8];
-        bf16x8 v[4];
-        f32x4 bias[8];                                   // of the unit's columns: 64 wave columns at a time, two units of columns per 32 rows
-        auto ask = [&](int half) __attribute__((always_inline)) {
+        const int64_t ldc = OUT == 2 ? part_ld(p.N) : p.ldc;
+        T* out = (OUT == 2 ? (T*)p.part + (int64_t)(kb0 / p.nk_split) * p.M * ldc : (T*)p.C) + row0 * ldc + col0;    // this lane's piece of the slab's rows 0 ... 7
+        typedef T __attribute__((ext_vector_type(4))) quad_t;
+        typedef T __attribute__((ext_vector_type(E))) piece_t;
+        constexpr int Q = UC / 8;                        // quads of a lane (its row, every eighth group of four columns)
+        quad_t o[Q];
+        piece_t v[4];
+        f32x4 bias[Q];                                   // of the unit's columns
+        auto ask = [&](int block) __attribute__((always_inline)) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) bias[k] = *reinterpret_cast<const f32x4*>(lds + bias_at + (wn * 128 + half * 64 + k * 8 + eh * 4) * 4);
+            for (int k = 0; k < Q; ++k)
+                if constexpr (OUT != 2) bias[k] = *reinterpret_cast<const f32x4*>(lds + bias_at + (wn * 128 + block * UC + k * 8 + eh * 4) * 4);
+                else bias[k] = f32x4{0.f, 0.f, 0.f, 0.f};
         };
         auto round = [&](auto uc) __attribute__((always_inline)) {
-            constexpr int U = decltype(uc)::value, I = U & 3, J = (U >> 2) * 2;           // column halves outside: each half's bias is read once
-            f32x16 &s0 = acc[I][J], &s1 = acc[I][J + 1];
-            asm volatile("" : "+a"(s0), "+a"(s1));       // fetched from the accumulation registers here, not all sums at the loop's end
+            constexpr int U = decltype(uc)::value, I = U & 3, J = (U >> 2) * (UC / 32);   // column blocks outside: each one's bias is read once
+            f32x16 &s0 = acc[I][J], &s1 = acc[I][EXACT ? J : J + 1];
+            asm volatile("" : "+a"(s0));                 // fetched from the accumulation registers here, not all sums at the loop's end
+            if constexpr (!EXACT) asm volatile("" : "+a"(s1));
 #pragma unroll
-            for (int k = 0; k < 8; ++k)
+            for (int k = 0; k < Q; ++k)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) o[k][e] = (bf16)((k < 4 ? s0 : s1)[4 * (k & 3) + e] + bias[k][e]);
+                for (int e = 0; e < 4; ++e) o[k][e] = (T)((k < 4 ? s0 : s1)[4 * (k & 3) + e] + bias[k][e]);
         };
         auto write = [&]() __attribute__((always_inline)) {
 #pragma unroll
-            for (int k = 0; k < 8; ++k) *reinterpret_cast<bf16x4*>(slab + e31 * 128 + (((k ^ e31) & 7) << 4) + eh * 8) = o[k];
+            for (int k = 0; k < Q; ++k)
+                if constexpr (EXACT) *reinterpret_cast<quad_t*>(slab + e31 * 128 + ((((2 * k + eh) ^ e31) & 7) << 4)) = o[k];
+                else *reinterpret_cast<quad_t*>(slab + e31 * 128 + (((k ^ e31) & 7) << 4) + eh * 8) = o[k];
         };
         auto read = [&]() __attribute__((always_inline)) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const bf16x8*>(slab + (k * 8 + (el >> 3)) * 128 + (((el ^ (el >> 3)) & 7) << 4));
+            for (int k = 0; k < 4; ++k) v[k] = *reinterpret_cast<const piece_t*>(slab + (k * 8 + (el >> 3)) * 128 + (((el ^ (el >> 3)) & 7) << 4));
         };
         auto store = [&](auto uc) __attribute__((always_inline)) {
-            constexpr int U = decltype(uc)::value, I = U & 3, C0 = (U >> 2) * 64;
-            typedef bf16 out_t __attribute__((ext_vector_type(8), aligned(2)));
+            constexpr int U = decltype(uc)::value, I = U & 3, C0 = (U >> 2) * UC;
+            typedef T out_t __attribute__((ext_vector_type(E), aligned(sizeof(T))));
             if (inside) {
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    out_t* c = reinterpret_cast<out_t*>(out + (I * 32 + k * 8) * p.ldc + C0);
+                    out_t* c = reinterpret_cast<out_t*>(out + (I * 32 + k * 8) * ldc + C0);
                     if constexpr (LINES) __builtin_nontemporal_store((out_t)v[k], c);
                     else *c = v[k];
                 }
             } else {
 #pragma unroll
                 for (int k = 0; k < 4; ++k)
-                    if (I * 32 + k * 8 < m_left && C0 < n_left) store_out<bf16, 8>(out + (I * 32 + k * 8) * p.ldc + C0, n_left - C0, v[k], false);
+                    if (I * 32 + k * 8 < m_left && C0 < n_left) store_out<T, E>(out + (I * 32 + k * 8) * ldc + C0, n_left - C0, v[k], false);
             }
         };
         auto unit = [&](auto uc) __attribute__((always_inline)) {
             constexpr int U = decltype(uc)::value;
-            if constexpr (U == 4) ask(1);
+            if constexpr ((U & 3) == 0) ask(U >> 2);
             round(uc);
             __builtin_amdgcn_sched_barrier(0);
             if constexpr (U > 0) store(std::integral_constant<int, U - 1>{});
@@ -542,18 +606,10 @@ __global__ __launch_bounds__(256, 1) void blocks_wide_kernel(const BlocksArgs p)
             __builtin_amdgcn_sched_barrier(0);
             read();                                      // (LDS operations of a wave keep their order)
         };
-        ask(0);
-        unit(std::integral_constant<int, 0>{});
-        unit(std::integral_constant<int, 1>{});
-        unit(std::integral_constant<int, 2>{});
-        unit(std::integral_constant<int, 3>{});
-        unit(std::integral_constant<int, 4>{});
-        unit(std::integral_constant<int, 5>{});
-        unit(std::integral_constant<int, 6>{});
-        unit(std::integral_constant<int, 7>{});
-        store(std::integral_constant<int, 7>{});
+        units(unit, std::make_integer_sequence<int, 4 * (128 / UC)>{});
+        store(std::integral_constant<int, 4 * (128 / UC) - 1>{});
         if (last) break;
-        stores = inside ? 32 : 0;
+        stores = inside ? 16 * (128 / UC) : 0;
         tile = next_tile;
         put_scales();                                    // every wave is behind its last read of the old words (a barrier per K-tile)
         bias_at = bias_at == WIDE_BIAS ? WIDE_BIAS + 1024 : WIDE_BIAS;
@@ -660,14 +716,11 @@ __global__ __launch_bounds__(256) void blocks_fold_kernel(const BlocksArgs p, in
     const int64_t n4 = (p.N + 3) / 4;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < p.M * n4; i += (int64_t)gridDim.x * 256) {
         const int64_t m = i / n4, n = i % n4 * 4, left = p.N - n;
-        typedef float vec_t __attribute__((ext_vector_type(4), aligned(4)));
         f32x4 s = {0.f, 0.f, 0.f, 0.f};
         for (int z = 0; z < splits; ++z) {
-            const float* c = p.part + ((int64_t)z * p.M + m) * p.N + n;
-            if (left >= 4) s += *reinterpret_cast<const vec_t*>(c);
-            else
+            const f32x4 c = *reinterpret_cast<const f32x4*>(p.part + ((int64_t)z * p.M + m) * part_ld(p.N) + n);
 #pragma unroll
-                for (int e = 0; e < 4; ++e) s[e] += e < left ? c[e] : 0.f;
+            for (int e = 0; e < 4; ++e) s[e] += e < left ? c[e] : 0.f;
         }
         T __attribute__((ext_vector_type(4))) o;
 #pragma unroll
@@ -684,14 +737,24 @@ struct BlocksPlan { int bm, bn, splits, nk_split; };
 // bf16 outputs take 256 x 256 tiles where those fill the 256 CUs and the reduction is long enough to pay for an epilogue nobody covers (us, 128 x 256 tiles : 256 x 256):
 //   101376 x 2304 x 384 139 : 138, x 512 161 : 139, x 768 224 : 200; 65536 x 768 x 768 55 : 49; 32768 x 4096 x 1024 159 : 142; 8192^3 513 : 400
 // With rows of C that start inside a 64-byte sector their 128-byte row pieces are written as parts of lines, past the caches or not: 101376 x 2296 x 768 225 : 306, and only a
-// long reduction hides it (30000 x 2296 x 2048 163 : 147, x 4096 297 : 254; 4099 x 50370 x 2048 467 : 476).  fp32 outputs gain nothing (the bf16 matrix instructions are the bound either way).
+// long reduction hides it (30000 x 2296 x 2048 163 : 147, x 4096 297 : 254; 4099 x 50370 x 2048 467 : 476).
+// fp32 outputs with such rows: 16384 x 4096 x 256 70 : 67, x 768 118 : 112; 8192^3 870 : 787; 4099 x 50304 x 768 344 : 322; with others not (4099 x 50370 x 768 374 : 458).  Added
+// onto what is there they stay with 128 x 256 (the wide epilogue has no time to wait for old values).  Their long reductions are split over 256 x 256 tiles where each workgroup gets
+// enough of them (128-row tiles, split as below : 256 x 256): 4096 x 1024 x 32768 238 : 209, 2304 x 768 x 101376 330 : 286, x 12544 62 : 59, 1024 x 1024 x 16384 58 : 52,
+// 2304 x 2304 x 8192 108 : 93; but where narrow tiles need no split, 2304 x 2304 x 4096, 55 : 61.
 // 128 x 256 where those fill the CUs twice; otherwise the reduction is split, or narrow tiles.
-BlocksPlan blocks_plan(int64_t M, int64_t N, int64_t K, bool out_bf16, bool whole_lines) {
+BlocksPlan blocks_plan(int64_t M, int64_t N, int64_t K, bool out_bf16, bool accumulate, bool whole_lines) {
     const int64_t tm = (M + 127) / 128, nk = K / 128;
     // straight from memory: 16 x 16, 32 x 16 or 64 x 32 outputs per workgroup
     const int mf = M <= 16 ? 1 : M <= 32 ? 2 : 4, nf = mf == 4 ? 2 : 1;
     if (nk <= 8 * direct_unroll(mf) * (mf == 1 ? 2 : 1) && (M + 16 * mf - 1) / (16 * mf) * ((N + 16 * nf - 1) / (16 * nf)) * (mf + nf) <= 3000) return {16 * mf, 16 * nf, 1, (int)nk};
     if (out_bf16 && nk >= (whole_lines ? 4 : 16) && ((M + 255) / 256) * ((N + 255) / 256) >= 256) return {256, 256, 1, (int)nk};
+    const int64_t tw = ((M + 255) / 256) * ((N + 255) / 256);
+    if (!out_bf16 && !accumulate && whole_lines && nk >= 2 && tw >= 256) return {256, 256, 1, (int)nk};
+    if (!out_bf16 && N > 128 && tw <= 128 && nk * tw / 256 >= (tw > 64 ? 16 : 8)) {
+        const int64_t s = 256 / tw, per = ((nk + s - 1) / s + 3) / 4 * 4;
+        if ((nk + per - 1) / per > 1) return {256, 256, (int)((nk + per - 1) / per), (int)per};
+    }
     if (N > 128 && tm * ((N + 255) / 256) >= 512) return {128, 256, 1, (int)nk};
     // a long reduction: split until there are about 512 workgroups, 24 blocks each at least with the wide tile, eight with the narrow one (fp32, narrow : wide:
     // 4096 x 1024 x 32768 251 : 236, 2304 x 768 x 101376 370 : 328; but 18 wide tiles, 768 x 768 x 65536, 92 : 102)
@@ -704,12 +767,26 @@ BlocksPlan blocks_plan(int64_t M, int64_t N, int64_t K, bool out_bf16, bool whol
     return {128, 128, 1, (int)nk};
 }
 
-template <int FA, bool LINES>
+template <typename T>
+void blocks_fold_launch(const BlocksArgs& p, hipStream_t s) {
+    const int64_t work = p.M * ((p.N + 3) / 4);
+    hipLaunchKernelGGL((blocks_fold_kernel<T>), dim3((unsigned)min((int64_t)4096, (work + 255) / 256)), dim3(256), 0, s, p, p.splits);
+}
+
+template <int FA, bool LINES, int OUT>
 int blocks_wide_launch(const BlocksArgs& p, hipStream_t s) {
-    const int tiles = p.ntm * p.ntn;
-    MERLOT_ENSURE_LDS((blocks_wide_kernel<FA, LINES>), WIDE_LDS, "merlot_gemm_f8_blocks");
-    hipLaunchKernelGGL((blocks_wide_kernel<FA, LINES>), dim3(tiles < 256 ? tiles : 256), dim3(256), WIDE_LDS, s, p);
+    const int items = p.ntm * p.ntn * p.splits;
+    MERLOT_ENSURE_LDS((blocks_wide_kernel<FA, LINES, OUT>), WIDE_LDS, "merlot_gemm_f8_blocks");
+    hipLaunchKernelGGL((blocks_wide_kernel<FA, LINES, OUT>), dim3(items < 256 ? items : 256), dim3(256), WIDE_LDS, s, p);
+    if (OUT == 2) blocks_fold_launch<float>(p, s);
     return MERLOT_OK;
+}
+
+template <int FA>
+int blocks_wide(const BlocksArgs& p, bool out_f32, bool lines, hipStream_t s) {
+    if (p.splits > 1) return blocks_wide_launch<FA, true, 2>(p, s);
+    if (out_f32) return blocks_wide_launch<FA, true, 1>(p, s);
+    return lines ? blocks_wide_launch<FA, true, 0>(p, s) : blocks_wide_launch<FA, false, 0>(p, s);
 }
 
 template <int FA, typename T>
@@ -721,17 +798,15 @@ void blocks_direct_launch(const BlocksArgs& p, int bm, hipStream_t s) {
 }
 
 template <int FA, int BN>
-void blocks_launch(const BlocksArgs& p, int splits, bool out_f32, hipStream_t s) {
-    const dim3 grid(p.ntm * p.ntn, splits), block(256);
-    if (splits > 1) {
-        const int64_t work = p.M * ((p.N + 3) / 4);
-        const dim3 fold((unsigned)min((int64_t)4096, (work + 255) / 256));
+void blocks_launch(const BlocksArgs& p, bool out_f32, hipStream_t s) {
+    const dim3 grid(p.ntm * p.ntn, p.splits), block(256);
+    if (p.splits > 1) {
         if (out_f32) {
             hipLaunchKernelGGL((blocks_gemm_kernel<FA, BN, 2, true>), grid, block, 0, s, p);
-            hipLaunchKernelGGL((blocks_fold_kernel<float>), fold, block, 0, s, p, splits);
+            blocks_fold_launch<float>(p, s);
         } else {
             hipLaunchKernelGGL((blocks_gemm_kernel<FA, BN, 2, false>), grid, block, 0, s, p);
-            hipLaunchKernelGGL((blocks_fold_kernel<bf16>), fold, block, 0, s, p, splits);
+            blocks_fold_launch<bf16>(p, s);
         }
     } else if (out_f32) {
         hipLaunchKernelGGL((blocks_gemm_kernel<FA, BN, 1, true>), grid, block, 0, s, p);
@@ -744,8 +819,9 @@ void blocks_launch(const BlocksArgs& p, int splits, bool out_f32, hipStream_t s)
 
 extern "C" int64_t merlot_gemm_f8_blocks_workspace_bytes(int64_t M, int64_t N, int64_t K) {
     if (M <= 0 || N <= 0 || K <= 0) return 0;
-    const BlocksPlan plan = blocks_plan(M, N, K, false, false);      // (wide tiles split nothing)
-    return plan.splits > 1 ? (int64_t)plan.splits * M * N * 4 : 0;
+    int splits = 1;                                      // whatever the output's type and alignment
+    for (int k = 0; k < 8; ++k) splits = max(splits, blocks_plan(M, N, K, k & 1, k & 2, k & 4).splits);
+    return splits > 1 ? (int64_t)splits * M * part_ld(N) * 4 : 0;
 }
 
 extern "C" int merlot_gemm_f8_blocks(const void* A8, int64_t lda, int fmt_a, const uint8_t* scale_a, int64_t ld_scale_a, const void* B8, int64_t ldb,
@@ -762,26 +838,25 @@ extern "C" int merlot_gemm_f8_blocks(const void* A8, int64_t lda, int fmt_a, con
                      (((uintptr_t)scale_a | (uintptr_t)scale_b) & 3) == 0,
                  MERLOT_EALIGN, "merlot_gemm_f8_blocks: scale rows must be 4-byte aligned and hold K / 128 bytes");
     const bool whole_lines = (((uintptr_t)C | (uint64_t)ldc * (out_f32 ? 4 : 2)) & 63) == 0;
-    const BlocksPlan plan = blocks_plan(M, N, K, !out_f32, whole_lines);
-    MERLOT_CHECK(plan.splits == 1 || (workspace && workspace_bytes >= (int64_t)plan.splits * M * N * 4), MERLOT_ESHAPE, "merlot_gemm_f8_blocks: workspace too small");
+    const BlocksPlan plan = blocks_plan(M, N, K, !out_f32, accumulate != 0, whole_lines);
+    MERLOT_CHECK(plan.splits == 1 || (workspace && workspace_bytes >= (int64_t)plan.splits * M * part_ld(N) * 4 && ((uintptr_t)workspace & 15) == 0), MERLOT_ESHAPE, "merlot_gemm_f8_blocks: workspace too small, or not 16-byte aligned");
     const int64_t ntm = (M + plan.bm - 1) / plan.bm, ntn = (N + plan.bn - 1) / plan.bn;
     MERLOT_CHECK(ntm * ntn < ((int64_t)1 << 24), MERLOT_ESHAPE, "merlot_gemm_f8_blocks: too many tiles");
     const BlocksArgs p = {(const uint8_t*)A8, (const uint8_t*)B8, scale_a, scale_b, lda, ldb, ld_scale_a, ld_scale_b, C, ldc, bias, (float*)workspace, M, N,
-                          (int)(K / 128), plan.nk_split, (int)ntm, (int)ntn, accumulate, (unsigned)(((uint64_t)1 << 32) / (4 * (uint64_t)ntn))};
+                          (int)(K / 128), plan.nk_split, plan.splits, (int)ntm, (int)ntn, accumulate, (unsigned)(((uint64_t)1 << 32) / (4 * (uint64_t)ntn))};
     hipStream_t s = (hipStream_t)stream;
     if (plan.bn <= 64) {
         if (out_f32) fmt_a == 0 ? blocks_direct_launch<0, float>(p, plan.bm, s) : blocks_direct_launch<1, float>(p, plan.bm, s);
         else fmt_a == 0 ? blocks_direct_launch<0, bf16>(p, plan.bm, s) : blocks_direct_launch<1, bf16>(p, plan.bm, s);
     } else if (plan.bm == 256) {
-        const int rc = fmt_a == 0 ? (whole_lines ? blocks_wide_launch<0, true>(p, s) : blocks_wide_launch<0, false>(p, s))
-                                  : (whole_lines ? blocks_wide_launch<1, true>(p, s) : blocks_wide_launch<1, false>(p, s));
+        const int rc = fmt_a == 0 ? blocks_wide<0>(p, out_f32 != 0, whole_lines, s) : blocks_wide<1>(p, out_f32 != 0, whole_lines, s);
         if (rc != MERLOT_OK) return rc;
     } else if (fmt_a == 0) {
-        if (plan.bn == 256) blocks_launch<0, 256>(p, plan.splits, out_f32 != 0, s);
-        else blocks_launch<0, 128>(p, plan.splits, out_f32 != 0, s);
+        if (plan.bn == 256) blocks_launch<0, 256>(p, out_f32 != 0, s);
+        else blocks_launch<0, 128>(p, out_f32 != 0, s);
     } else {
-        if (plan.bn == 256) blocks_launch<1, 256>(p, plan.splits, out_f32 != 0, s);
-        else blocks_launch<1, 128>(p, plan.splits, out_f32 != 0, s);
+        if (plan.bn == 256) blocks_launch<1, 256>(p, out_f32 != 0, s);
+        else blocks_launch<1, 128>(p, out_f32 != 0, s);
     }
     return merlot_launch_status("merlot_gemm_f8_blocks");
 }
