@@ -5,6 +5,8 @@
 //
 // Both directions are bound by memory: every operand crosses it once.  A row is held in registers by WPR waves (1 up to 2 048 features, 4 above), each lane
 // VEC consecutive features per slab, so a lane's loads and stores are 8 or 16 bytes and the 128 features that share a scale lie in 128 / VEC neighbouring lanes.
+// Measured (101376 x 768 bf16): forward with residual 114 us = 5.45 TB/s (a large copy: 4.85 TB/s), with the 8-bit copy in place of y 103 us, backward with
+// the residual stream's gradient 120 us + 5 us for dgamma = 5.0 TB/s.  Widths that are whole slabs take code without per-element branches (FULL: backward 184 -> 120 us).
 // All sums are fp32.  The statistics are taken from h AS STORED (rounded to its type), so that the backward, which reads the stored h, differentiates the
 // function the forward computed.
 #include "common.h"
@@ -249,6 +251,7 @@ constexpr int RMS_MAX_H = 16384;
 
 int rms_rows_per_block(int H) { return H <= 2048 ? 4 : 1; }
 
+// 1 024 workgroups: 101376 x 768 takes 160 us with 512, 121 with 1 024, 134 with 2 048 (more partial rows to write and add up)
 int rms_bwd_blocks(int64_t rows, int H) {
     const int64_t nb = (rows + rms_rows_per_block(H) - 1) / rms_rows_per_block(H);
     return (int)(nb < 1024 ? nb : 1024);

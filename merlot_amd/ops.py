@@ -3,6 +3,8 @@
 PyTorch is plumbing only: it owns device memory and the stream; every op below is one or more
 hand-written gfx950 kernels in libmerlot_hip.so.  There is no eager / CPU fallback.
 """
+import functools
+
 import torch
 
 from .lib import call, LIB
@@ -42,9 +44,9 @@ def _p(t):
     return None if t is None else t.data_ptr()
 
 
-def _stream():
+def _stream(dev=None):
     # the raw handle of torch.cuda.current_stream(), without the Stream object around it (0.3 us instead of 2.7 us per launch)
-    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device() if dev is None else dev)
 
 
 _NT_WS = {}
@@ -901,34 +903,49 @@ def weight_std_bwd(dkhat_t, khat, rstd, gk2d):
 
 
 # ---- root-mean-square norm, 8-bit blocks, gradient clipping ------------------------------------------------------------------
-def _operands(*operands):
-    """(tensor or None, dtype, name) each: a GPU tensor of that type with a contiguous last dimension (_chk), all on the CURRENT device (the library launches on the
-    current device's stream)"""
-    dev = None
-    for t, dtype, name in operands:
-        if t is None:
-            continue
-        if dev is None:
-            dev = torch.cuda.current_device() if t.is_cuda else -2
-        if t.dtype is not dtype or t.get_device() != dev or t.dim() == 0 or t.stride(-1) != 1:
-            _chk(t, dtype, name)
-            raise ValueError(f"{name}: on {t.device} while the current device is cuda:{dev}: call under torch.cuda.device({t.get_device()})")
+def _device(t, name):
+    """the device of a GPU tensor, which has to be the CURRENT one (the library launches on the current device's stream)"""
+    dev = t.get_device()
+    if dev < 0:
+        raise ValueError(f"{name}: expected a GPU tensor (the HIP path has no CPU fallback)")
+    if dev != torch.cuda.current_device():
+        raise ValueError(f"{name}: on {t.device} while the current device is cuda:{torch.cuda.current_device()}: call under torch.cuda.device({dev})")
+    return dev
 
 
-def _rows(t, name):
-    """(2-D view, row stride): any leading dims where they collapse without a copy; rows may be further apart than they are long, not nearer"""
-    if t.dim() != 2:
+def _rows(t, dtype, dev, name):
+    """(rows, columns, row stride) of a tensor of that type on that device: any leading dims where they collapse without a copy; rows may be further apart than they
+    are long, not nearer"""
+    if t.dtype is not dtype:
+        raise ValueError(f"{name}: expected dtype {dtype}, got {t.dtype}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name}: expected a tensor on cuda:{dev}, the current device, got {t.device}")
+    strides = t.stride()
+    if not strides or strides[-1] != 1:
+        raise ValueError(f"{name}: last dim must be contiguous")
+    if len(strides) != 2:
+        cols = t.shape[-1]
         try:
-            t = t.view(-1, t.shape[-1]) if t.numel() else t.reshape(0, t.shape[-1])
+            t = t.view(-1, cols) if t.numel() else t.reshape(0, cols)
         except RuntimeError:
             raise ValueError(f"{name}: leading dimensions do not collapse into rows without a copy") from None
+        strides = t.stride()
     rows, cols = t.shape
     if rows <= 1:
-        return t, cols
-    ld = t.stride(0)
-    if ld < cols:
-        raise ValueError(f"{name}: rows overlap (stride {ld}, {cols} columns)")
-    return t, ld
+        return rows, cols, cols
+    if strides[0] < cols:
+        raise ValueError(f"{name}: rows overlap (stride {strides[0]}, {cols} columns)")
+    return rows, cols, strides[0]
+
+
+def _dense(t, n, dev, name):
+    """n dense f32 values on that device"""
+    if t.dtype is not F32:
+        raise ValueError(f"{name}: expected dtype {F32}, got {t.dtype}")
+    if t.get_device() != dev:
+        raise ValueError(f"{name}: expected a tensor on cuda:{dev}, the current device, got {t.device}")
+    if t.shape != (n,) or not t.is_contiguous():
+        raise ValueError(f"{name}: expected [{n}], dense, got {tuple(t.shape)}")
 
 
 def _scales8(rows, cols, like):
@@ -943,54 +960,58 @@ def rms_norm_fwd(x, gamma, *, residual=None, out=True, q8=False, save_rstd=True,
     x [..., H] bf16 or f32, residual like x (or None: h is x), gamma f32 [H].  -> (y, h, rstd, y8, scale8): y like x (None: out False); h None without a
     residual; rstd f32 [rows] (None: save_rstd False); q8: y8 / scale8 = the e4m3 copy of the unrounded y in blocks of 128 features, as quantize_blocks
     lays it out -- the left operand of gemm_f8_blocks."""
-    if x.dtype not in (BF16, F32):
-        raise ValueError(f"x: expected bf16 or f32, got {x.dtype}")
-    _operands((x, x.dtype, 'x'), (gamma, F32, 'gamma'), (residual, x.dtype, 'residual'))
-    x2, ldx = _rows(x, 'x')
-    rows, H = x2.shape
-    if gamma.shape != (H,):
-        raise ValueError(f"gamma: expected [{H}], got {tuple(gamma.shape)}")
-    if residual is not None and residual.shape != x.shape:
-        raise ValueError(f"residual: expected {tuple(x.shape)}, got {tuple(residual.shape)}")
+    dt = x.dtype
+    if dt is not BF16 and dt is not F32:
+        raise ValueError(f"x: expected bf16 or f32, got {dt}")
+    dev = _device(x, 'x')
+    rows, H, ldx = _rows(x, dt, dev, 'x')
+    _dense(gamma, H, dev, 'gamma')
     if not out and not q8:
         raise ValueError("rms_norm_fwd: neither out nor q8 is asked for")
-    r2, ldr = _rows(residual, 'residual') if residual is not None else (None, 0)
-    y = x.new_empty(x.shape) if out else None
-    h = x.new_empty(x.shape) if residual is not None else None
+    shape = x.shape
+    h = ldr = 0
+    if residual is None:
+        h = None
+    else:
+        if residual.shape != shape:
+            raise ValueError(f"residual: expected {tuple(shape)}, got {tuple(residual.shape)}")
+        ldr = _rows(residual, dt, dev, 'residual')[2]
+        h = x.new_empty(shape)
+    y = x.new_empty(shape) if out else None
     rstd = gamma.new_empty(rows) if save_rstd else None
     y8 = s8 = None
     if q8:
         y8 = x.new_empty((rows, (H + 127) // 128 * 128), dtype=FP8)
         s8 = _scales8(rows, H, x)
     if rows:
-        call('merlot_rms_fwd', x2.data_ptr(), ldx, 1 if x.dtype is F32 else 0, _p(r2), ldr, gamma.data_ptr(), _p(h), _p(y), _p(rstd), _p(y8),
-             (H + 127) // 128 * 128, _p(s8), (H + 511) // 512 * 4, rows, H, eps, _stream())
+        call('merlot_rms_fwd', x.data_ptr(), ldx, 1 if dt is F32 else 0, _p(residual), ldr, gamma.data_ptr(), _p(h), _p(y), _p(rstd), _p(y8),
+             (H + 127) // 128 * 128, _p(s8), (H + 511) // 512 * 4, rows, H, eps, _stream(dev))
     return y, h, rstd, y8, s8
 
 
 def rms_norm_bwd(dy, h, rstd, gamma, dgamma, *, dres=None):
     """gradient of rms_norm_fwd: h (x where there was no residual) and rstd as the forward left them, dy the gradient of y, dres that of h from elsewhere (the
     residual stream).  -> dx, which is the residual's gradient too; dgamma f32 [H] is ACCUMULATED, in a fixed order (the same call gives the same bits)."""
-    if h.dtype not in (BF16, F32):
-        raise ValueError(f"h: expected bf16 or f32, got {h.dtype}")
-    _operands((h, h.dtype, 'h'), (dy, h.dtype, 'dy'), (dres, h.dtype, 'dres'), (rstd, F32, 'rstd'), (gamma, F32, 'gamma'), (dgamma, F32, 'dgamma'))
-    h2, ldh = _rows(h, 'h')
-    rows, H = h2.shape
+    dt = h.dtype
+    if dt is not BF16 and dt is not F32:
+        raise ValueError(f"h: expected bf16 or f32, got {dt}")
+    dev = _device(h, 'h')
+    rows, H, ldh = _rows(h, dt, dev, 'h')
+    shape = h.shape
     for t, nm in ((dy, 'dy'), (dres, 'dres')):
-        if t is not None and t.shape != h.shape:
-            raise ValueError(f"{nm}: expected {tuple(h.shape)}, got {tuple(t.shape)}")
-    if gamma.shape != (H,) or dgamma.shape != (H,):
-        raise ValueError(f"gamma, dgamma: expected [{H}], got {tuple(gamma.shape)}, {tuple(dgamma.shape)}")
-    if rstd.numel() != rows or not rstd.is_contiguous():
-        raise ValueError(f"rstd: expected {rows} dense values")
-    dy2, lddy = _rows(dy, 'dy')
-    dr2, lddr = _rows(dres, 'dres') if dres is not None else (None, 0)
-    dx = h.new_empty(h.shape)
+        if t is not None and t.shape != shape:
+            raise ValueError(f"{nm}: expected {tuple(shape)}, got {tuple(t.shape)}")
+    lddy = _rows(dy, dt, dev, 'dy')[2]
+    lddr = 0 if dres is None else _rows(dres, dt, dev, 'dres')[2]
+    _dense(gamma, H, dev, 'gamma')
+    _dense(dgamma, H, dev, 'dgamma')
+    _dense(rstd, rows, dev, 'rstd')
+    dx = h.new_empty(shape)
     if rows:
         nbytes = LIB.query('merlot_rms_bwd_workspace_bytes', rows, H)
         ws = gamma.new_empty(nbytes // 4)
-        call('merlot_rms_bwd', _p(dy2), lddy, 1 if h.dtype == F32 else 0, _p(h2), ldh, _p(rstd), _p(gamma), _p(dr2), lddr, _p(dx), _p(dgamma), rows, H,
-             _p(ws), nbytes, _stream())
+        call('merlot_rms_bwd', dy.data_ptr(), lddy, 1 if dt is F32 else 0, h.data_ptr(), ldh, rstd.data_ptr(), gamma.data_ptr(), _p(dres), lddr, dx.data_ptr(),
+             dgamma.data_ptr(), rows, H, ws.data_ptr(), nbytes, _stream(dev))
     return dx
 
 
@@ -999,17 +1020,16 @@ def quantize_blocks(x, fmt=F8_E4M3, *, tile=1, rows=True, transpose=False):
     q [R, C padded with zeros to whole blocks] float8, s [R, blocks] uint8: a byte b stands for 2^(b - 127), the least power of two that brings the block's max |x|
     to the format's largest value or under it; 255 = NaN, for a block that holds an infinity or NaN.  qt / st: the same of x^T, blocks along x's rows.
     tile=128: one scale per 128 x 128 tile (weights: q and qt then hold the same values).  fmt: F8_E4M3 or F8_E5M2."""
-    if x.dtype not in (BF16, F32):
+    if x.dtype is not BF16 and x.dtype is not F32:
         raise ValueError(f"x: expected bf16 or f32, got {x.dtype}")
-    _operands((x, x.dtype, 'x'))
+    dev = _device(x, 'x')
     if x.dim() != 2 or x.shape[1] == 0:
         raise ValueError(f"x: expected [rows, columns >= 1], got {tuple(x.shape)}")
     if fmt not in _F8_DTYPES or tile not in (1, 128):
         raise ValueError("quantize_blocks: fmt must be F8_E4M3 or F8_E5M2, tile 1 or 128")
     if not rows and not transpose:
         raise ValueError("quantize_blocks: neither rows nor transpose is asked for")
-    x2, ldx = _rows(x, 'x')
-    R, C = x.shape
+    R, C, ldx = _rows(x, x.dtype, dev, 'x')
     dt = _F8_DTYPES[fmt]
     q = s = qt = st = None
     if rows:
@@ -1017,56 +1037,67 @@ def quantize_blocks(x, fmt=F8_E4M3, *, tile=1, rows=True, transpose=False):
     if transpose:
         qt, st = x.new_empty((C, (R + 127) // 128 * 128), dtype=dt), _scales8(C, R, x)
     if R:
-        call('merlot_quantize_blocks', x2.data_ptr(), ldx, 1 if x.dtype is F32 else 0, R, C, fmt, tile, _p(q), (C + 127) // 128 * 128, _p(s), (C + 511) // 512 * 4,
-             _p(qt), (R + 127) // 128 * 128, _p(st), (R + 511) // 512 * 4, _stream())
+        call('merlot_quantize_blocks', x.data_ptr(), ldx, 1 if x.dtype is F32 else 0, R, C, fmt, tile, _p(q), (C + 127) // 128 * 128, _p(s), (C + 511) // 512 * 4,
+             _p(qt), (R + 127) // 128 * 128, _p(st), (R + 511) // 512 * 4, _stream(dev))
     return (q, s, qt, st) if transpose else (q, s)
 
 
-def _scale_ld(s, rows, nb, name):
-    if s.shape != (rows, nb):
-        raise ValueError(f"{name}: expected [{rows}, {nb}] scale bytes, got {tuple(s.shape)}")
-    ld = (nb + 3) // 4 * 4 if rows <= 1 else s.stride(0)
-    if rows and s.storage_offset() + (rows - 1) * ld + (nb + 3) // 4 * 4 > s.untyped_storage().nbytes():
+def _scale_rows(s, rows, nb, dev, name):
+    """row stride of `rows` rows of nb scale bytes, read in whole words of 4"""
+    if s.dtype is not torch.uint8 or s.get_device() != dev or s.shape != (rows, nb):
+        raise ValueError(f"{name}: expected [{rows}, {nb}] scale bytes (uint8) on cuda:{dev}, got {tuple(s.shape)} {s.dtype} on {s.device}")
+    ld, one = s.stride()
+    if one != 1:
+        raise ValueError(f"{name}: last dim must be contiguous")
+    whole = (nb + 3) // 4 * 4
+    if rows <= 1:
+        ld = whole
+    if nb != whole and rows and s.storage_offset() + (rows - 1) * ld + whole > s.untyped_storage().nbytes():
         raise ValueError(f"{name}: rows are read in whole words of 4 bytes, the last one ends before its word does")
     return ld
+
+
+@functools.lru_cache(maxsize=4096)
+def _gemm_f8_blocks_workspace(M, N, K):                  # (a function of the sizes alone)
+    return LIB.query('merlot_gemm_f8_blocks_workspace_bytes', M, N, K)
 
 
 def gemm_f8_blocks(a8, a_scale, b8, b_scale, *, bias=None, out=None, out_dtype=BF16, accumulate=False):
     """C[M,N] (+)= a8[M,K] @ b8[N,K]^T (+ bias) on 8-bit operands with a scale per row and block of 128, as quantize_blocks / rms_norm_fwd(q8=True) make them: a8 e4m3
     or e5m2, b8 e4m3, K a multiple of 128, row strides under 2^22; M, N any.  fp32 accumulation; C bf16 or f32 (out / out_dtype), accumulate (f32 out only) adds into out."""
-    fa = 1 if a8.dtype == torch.float8_e5m2 else 0
-    _operands((a8, _F8_DTYPES[fa], 'a8'), (b8, FP8, 'b8'), (a_scale, torch.uint8, 'a_scale'), (b_scale, torch.uint8, 'b_scale'), (bias, F32, 'bias'))
-    if a8.dim() != 2 or b8.dim() != 2 or a8.shape[1] != b8.shape[1] or a8.shape[1] == 0 or a8.shape[1] % 128 != 0:
+    dt = a8.dtype
+    fa = 1 if dt is torch.float8_e5m2 else 0
+    dev = _device(a8, 'a8')
+    if a8.dim() != 2 or b8.dim() != 2:
         raise ValueError(f"gemm_f8_blocks: operands [M, K] and [N, K] with K a multiple of 128, got {tuple(a8.shape)} and {tuple(b8.shape)}")
-    M, K = a8.shape
-    N = b8.shape[0]
-    _, lda = _rows(a8, 'a8')
-    _, ldb = _rows(b8, 'b8')
-    ldsa, ldsb = _scale_ld(a_scale, M, K // 128, 'a_scale'), _scale_ld(b_scale, N, K // 128, 'b_scale')
-    if bias is not None and bias.shape != (N,):
-        raise ValueError(f"bias: expected [{N}], got {tuple(bias.shape)}")
+    M, K, lda = _rows(a8, _F8_DTYPES[fa], dev, 'a8')
+    N, Kb, ldb = _rows(b8, FP8, dev, 'b8')
+    if K != Kb or K == 0 or K % 128 != 0:
+        raise ValueError(f"gemm_f8_blocks: operands [M, K] and [N, K] with K a multiple of 128, got {tuple(a8.shape)} and {tuple(b8.shape)}")
+    ldsa, ldsb = _scale_rows(a_scale, M, K // 128, dev, 'a_scale'), _scale_rows(b_scale, N, K // 128, dev, 'b_scale')
+    if bias is not None:
+        _dense(bias, N, dev, 'bias')
     if out is None:
         if accumulate:
             raise ValueError("gemm_f8_blocks: accumulate needs out")
-        if out_dtype not in (BF16, F32):
+        if out_dtype is not BF16 and out_dtype is not F32:
             raise ValueError(f"out_dtype: expected bf16 or f32, got {out_dtype}")
+        f32 = out_dtype is F32
         out = a8.new_empty((M, N), dtype=out_dtype)
         ldc = N
     else:
-        if out.dtype not in (BF16, F32) or out.shape != (M, N):
+        f32 = out.dtype is F32
+        if not f32 and out.dtype is not BF16 or out.shape != (M, N):
             raise ValueError(f"out: expected bf16 or f32 [{M}, {N}], got {out.dtype} {tuple(out.shape)}")
-        if accumulate and out.dtype != F32:
+        if accumulate and not f32:
             raise ValueError("gemm_f8_blocks: accumulate needs an f32 out")
-        if M and N:
-            _operands((out, out.dtype, 'out'))
-            _, ldc = _rows(out, 'out')
+        ldc = _rows(out, out.dtype, dev, 'out')[2] if M and N else N
     if M == 0 or N == 0:
         return out
-    nbytes = LIB.query('merlot_gemm_f8_blocks_workspace_bytes', M, N, K)
+    nbytes = _gemm_f8_blocks_workspace(M, N, K)
     ws = a8.new_empty(nbytes // 4, dtype=F32) if nbytes else None   # caller-owned partial products of a split reduction
-
-    args = (_p(a8), lda, fa, _p(a_scale), ldsa, _p(b8), ldb, _p(b_scale), ldsb, _p(out), ldc, M, N, K, 1 if out.dtype == F32 else 0, 1 if accumulate else 0,
-            _p(bias), _p(ws), nbytes, _stream())
+    args = (a8.data_ptr(), lda, fa, a_scale.data_ptr(), ldsa, b8.data_ptr(), ldb, b_scale.data_ptr(), ldsb, out.data_ptr(), ldc, M, N, K, 1 if f32 else 0,
+            1 if accumulate else 0, _p(bias), _p(ws), nbytes, _stream(dev))
     if TIMER is not None:
         TIMER.time('gemm_f8_blocks', 2.0 * M * N * K, lambda: call('merlot_gemm_f8_blocks', *args))
     else:
