@@ -6,7 +6,7 @@
 // as kernel arguments, those of more than 112 tensors by way of small launches that write them into a table in the workspace -- nothing to copy, nothing kept from one call
 // for the next, and a captured call replays as it is.  Squares are summed in 64 bits (a model's 2 * 10^8 addends; half the fp32 rate is far above what memory
 // delivers) in a fixed order: each workgroup leaves one partial, every workgroup of the second pass adds all partials up by itself (8 KiB from the L2), which
-// saves the launch between the passes.  Measured: one buffer of 223 M fp32 values 149 us (6.0 TB/s) + 323 us (5.5 TB/s), 300 tensors of 60 M values in all 182 us.
+// saves the launch between the passes.  Measured: one buffer of 223 M fp32 values 149 us (6.0 TB/s) + 323 us (5.5 TB/s), 300 tensors of 60 M values in all 141 us.
 #include <stdlib.h>
 #include <algorithm>
 #include "common.h"
@@ -111,7 +111,6 @@ template <typename TI, typename TO>
 __device__ __forceinline__ void clip_scale(const TI* g, TO* out, int64_t n, uint32_t chunk, float coef) {
     constexpr int E = 16 / sizeof(TI), U = CLIP_CHUNK / E / 256;
     const int shift = clip_shift<TI>(g);
-    const bool wide = ((uintptr_t)(out - shift) & 15) == 0;      // the output's groups are aligned where the input's are
     const int64_t first = (int64_t)chunk * (CLIP_CHUNK / E);
     float v[U][E];
 #pragma unroll
@@ -119,8 +118,9 @@ __device__ __forceinline__ void clip_scale(const TI* g, TO* out, int64_t n, uint
 #pragma unroll
     for (int u = 0; u < U; ++u) {
         const int64_t i0 = (first + u * 256 + threadIdx.x) * E - shift;
-        if (wide && i0 >= 0 && i0 + E <= n) {
-            typedef TO vec_t __attribute__((ext_vector_type(E), aligned(8)));
+        if (i0 >= 0 && i0 + E <= n) {
+            // whole groups wherever the output starts (gfx950 stores global dwords at byte alignment): 300 outputs packed into one buffer, 60 M values, 188 -> 141 us
+            typedef TO vec_t __attribute__((ext_vector_type(E), aligned(sizeof(TO))));
             vec_t o;
 #pragma unroll
             for (int e = 0; e < E; ++e) o[e] = (TO)(v[u][e] * coef);

@@ -61,6 +61,23 @@ def test_mixed_tensors(sizes, clip, shift):
         assert all(torch.equal(d.cpu(), t) for t, d in zip(host, dev))
 
 
+@pytest.mark.parametrize('into', [F, B])
+@pytest.mark.parametrize('kind', [F, B])
+def test_outputs_at_any_offset(kind, into):
+    """inputs and outputs that start at different places of their 16 bytes; nothing beside the outputs is written"""
+    ops = _ops()
+    sizes = [9, 4096, 5001, 12289, 700, 33, 8192, 20000, 15]
+    host, dev, _ = _tensors(sizes, [kind] * len(sizes), 3, 0.1, 1)
+    bases = [torch.full((n + 32,), 7.0, device='cuda', dtype=into) for n in sizes]
+    for first in (0, 1, 2, 5):
+        outs = [b[(first + 3 * i) % 8:][:n] for i, (b, n) in enumerate(zip(bases, sizes))]
+        _check(host, outs, ops.clip_by_global_norm(dev, 2.0, out=outs), 2.0, [into] * len(sizes))
+        for i, (b, n) in enumerate(zip(bases, sizes)):
+            s = (first + 3 * i) % 8
+            assert bool((b[:s] == 7).all()) and bool((b[s + n:] == 7).all())
+            b.fill_(7.0)
+
+
 def test_more_tensors_than_one_launch_takes_and_a_kept_list():
     ops = _ops()
     sizes = [1 + (i * 37) % 1500 for i in range(300)]
