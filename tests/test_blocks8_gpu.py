@@ -160,12 +160,53 @@ def test_large_products_of_whole_numbers_are_exact(M, N, K, fa):
     want = va @ vb.t() + bias
     assert float((va.abs() @ vb.abs().t()).max()) + 50 < 2 ** 24
     for dt in (torch.bfloat16, torch.float32):
-        buf = torch.full((M + 1, N), 7.0, device='cuda', dtype=dt)
-        got = ops.gemm_f8_blocks(a, sa, b, sb, bias=bias, out=buf[:M])
-        assert torch.equal(got, want.to(dt)), dt
-        assert bool((buf[M] == 7).all())
+        for pad in (0, 32, 5):                                 # rows of C further apart than they are long: on whole sectors, and not
+            buf = torch.full((M + 1, N + pad), 7.0, device='cuda', dtype=dt)
+            got = ops.gemm_f8_blocks(a, sa, b, sb, bias=bias, out=buf[:M, :N])
+            assert torch.equal(got, want.to(dt)), (dt, pad)
+            assert bool((buf[M] == 7).all()) and bool((buf[:, N:] == 7).all())
     c = torch.randint(-9, 9, (M, N), device='cuda').float()
     assert torch.equal(ops.gemm_f8_blocks(a, sa, b, sb, out=c.clone(), accumulate=True), c + (want - bias))
+
+
+def test_offsets_past_32_bits():
+    """operands, copies and outputs of more than 4 GiB: their last rows against the same rows alone"""
+    ops = _ops()
+    rows, K = (1 << 22) + 300, 1024
+    x = torch.zeros(rows, K, device='cuda', dtype=torch.bfloat16)
+    tail = _x(600, K, torch.bfloat16, 1).cuda()
+    x[-600:] = tail
+    w8, sw = ops.quantize_blocks(_x(70, K, torch.bfloat16, 2).cuda(), tile=128)
+    gamma = torch.rand(K, device='cuda')
+    x8, sx = ops.quantize_blocks(x)
+    t8, st = ops.quantize_blocks(tail)
+    assert torch.equal(x8[-600:].view(torch.uint8), t8.view(torch.uint8)) and torch.equal(sx[-600:], st)
+    assert torch.equal(ops.gemm_f8_blocks(x8, sx, w8, sw)[-600:], ops.gemm_f8_blocks(x8[-600:], sx[-600:], w8, sw))
+    want = ops.gemm_f8_blocks(t8, st, w8, sw, out_dtype=torch.float32)
+    got = ops.gemm_f8_blocks(x8, sx, w8, sw, out_dtype=torch.float32)[-600:]
+    mag = ref.values(t8, st).cuda().abs() @ ref.values(w8, sw).cuda().abs().t().contiguous()
+    assert bool(((got - want).abs() <= 2 * (K + 64) * 2.0 ** -23 * mag).all())          # (other tiles: sums in another order, each within its own tolerance)
+    xt8, sxt = ops.quantize_blocks(x, rows=False, transpose=True)[2:]                   # [1024, 4.2 M]: blocks along the rows
+    b0 = (rows - 600) // 128 + 1
+    q, s = ops.quantize_blocks(x[b0 * 128:], rows=False, transpose=True)[2:]
+    assert torch.equal(xt8[:, b0 * 128:].view(torch.uint8), q.view(torch.uint8)) and torch.equal(sxt[:, b0:], s)
+    del x8, sx, xt8, sxt
+    y, _, r, y8, s8 = ops.rms_norm_fwd(x, gamma, q8=True)
+    yt, _, rt, y8t, s8t = ops.rms_norm_fwd(tail, gamma, q8=True)
+    assert torch.equal(y[-600:], yt) and torch.equal(r[-600:], rt) and torch.equal(y8[-600:].view(torch.uint8), y8t.view(torch.uint8)) and torch.equal(s8[-600:], s8t)
+    dg, dgt = torch.zeros_like(gamma), torch.zeros_like(gamma)
+    dx = ops.rms_norm_bwd(x, x, r, gamma, dg)
+    assert torch.equal(dx[-600:], ops.rms_norm_bwd(tail, tail, rt, gamma, dgt))
+    mag = (tail.double().square() * rt.double().unsqueeze(1)).sum(0)
+    assert bool(((dg.double() - dgt).abs() <= 2 * (600 + 8) * 2.0 ** -23 * mag).all())  # the other rows add zeros: 600 addends in two orders
+    del x, y, y8, s8, dx
+    M, N = 66000, 33000
+    a, sa, va = _whole_on_device(M, 128, 0, 3)
+    b, sb, vb = _whole_on_device(N, 128, 0, 4)
+    for dt in (torch.bfloat16, torch.float32):
+        got = ops.gemm_f8_blocks(a, sa, b, sb, out_dtype=dt)
+        assert torch.equal(got[-300:], (va[-300:] @ vb.t()).to(dt)) and torch.equal(got[:300], (va[:300] @ vb.t()).to(dt))
+        del got
 
 
 @pytest.mark.parametrize('N', [3, 300, 5000])
