@@ -286,8 +286,8 @@ __global__ __launch_bounds__(256, 2) void blocks_gemm_kernel(const BlocksArgs p)
 // Large outputs: 256 x 256 tiles, four waves of 128 x 128 -- ONE per SIMD, 256 accumulators each --, K-tiles of 128 (whole 128-byte lines per row, where 64-byte steps
 // ask the L2 twice per line), two K-tile buffers.  A wave's next fragments are read, and the next K-tile is fetched, between its own matrix instructions; the one barrier
 // per K-tile stands where the buffer's last reads have returned.  Persistent: workgroups walk the tiles of their XCD's band, the fetch stream runs on across tile ends, and
-// a tile's stores drain while the next one multiplies.  fp32 outputs convert two fragment slices between every four matrix instructions: with 128 x 128 per wave that is two
-// conversions a matrix instruction, with 64 x 128 three (8192^3: 787 us = 1.4 PFLOP/s, the rate of a large bf16 product, against 870).
+// a tile's stores drain while the next one multiplies.  fp32 outputs convert two fragment slices between every four matrix
+// instructions, two conversions each (8192^3: 745 - 787 us = 1.4 - 1.5 PFLOP/s, the rate of a large bf16 product; 128 x 256 tiles 870).
 constexpr int WIDE_BUF = 65536, WIDE_SCALES = 2 * WIDE_BUF, WIDE_BIAS = WIDE_SCALES + 512 * SCALE_BLOCKS, WIDE_SLAB = WIDE_BIAS + 2048;
 constexpr int WIDE_LDS = WIDE_SLAB + 4 * 4096;           // two K-tiles, 16 blocks' scale bytes of 512 rows, two tiles' bias, a slab of 32 rows x 128 bytes per wave
 
