@@ -17,36 +17,71 @@ namespace {
 // VEC consecutive elements at any element alignment (gfx950 loads and stores global dwords at byte alignment): rows of odd width need no path of their own
 template <typename T, int VEC> struct ElemVec { typedef T type __attribute__((ext_vector_type(VEC), aligned(sizeof(T)))); };
 
-// `left`: how many of the VEC elements exist (may be <= 0); FULL: all of them do, the width is a whole number of slabs
-template <typename T, int VEC, bool FULL>
-__device__ __forceinline__ void load_vec(const T* p, int left, float (&v)[VEC]) {
-    if (FULL || left >= VEC) {
-        const typename ElemVec<T, VEC>::type t = *reinterpret_cast<const typename ElemVec<T, VEC>::type*>(p);
+// elements c ... c + VEC - 1 of a row of H; those past its end are zeros and are not stored.  FULL: H is a whole number of slabs.  base: the slab's first element, the same
+// in every lane -- whole slabs take no checks.  In the slab that the row's end lies in every lane loads one vector all the same, the lane at the end the row's last VEC elements,
+// which it moves down (50000 x 2000 bf16: element by element the backward took 267 us, this way RMS_ODD).
+template <typename T, int VEC, bool FULL, int SLAB>
+__device__ __forceinline__ void load_vec(const T* row, int base, int c, int H, float (&v)[VEC]) {
+    typedef typename ElemVec<T, VEC>::type vec_t;
+    if (FULL || base + SLAB <= H) {
+        const vec_t t = *reinterpret_cast<const vec_t*>(row + c);
 #pragma unroll
         for (int e = 0; e < VEC; ++e) v[e] = (float)t[e];
+    } else if (base >= H) {
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = 0.f;
+    } else if (H >= VEC) {
+        const int left = H - c;
+        const vec_t t = *reinterpret_cast<const vec_t*>(row + (left >= VEC ? c : left > 0 ? H - VEC : 0));
+        const int s = left >= VEC ? 0 : VEC - left;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) v[e] = left > 0 ? (float)t[e] : 0.f;
+#pragma unroll
+        for (int b = 1; b < VEC; b *= 2)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] = left > 0 && (s & b) ? (e + b < VEC ? v[e + b] : 0.f) : v[e];
     } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = e < left ? (float)p[e] : 0.f;
+        for (int e = 0; e < VEC; ++e) v[e] = c + e < H ? (float)row[c + e] : 0.f;
     }
 }
-template <typename T, int VEC, bool FULL>
-__device__ __forceinline__ void store_vec(T* p, int left, const float (&v)[VEC]) {
-    if (FULL || left >= VEC) {
-        typename ElemVec<T, VEC>::type t;
+template <typename T, int VEC, bool FULL, int SLAB>
+__device__ __forceinline__ void store_vec(T* row, int base, int c, int H, const float (&v)[VEC]) {
+    typedef typename ElemVec<T, VEC>::type vec_t;
+    vec_t t;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) t[e] = (T)v[e];
-        *reinterpret_cast<typename ElemVec<T, VEC>::type*>(p) = t;
-    } else {
+    for (int e = 0; e < VEC; ++e) t[e] = (T)v[e];
+    if (FULL || base + SLAB <= H || H - c >= VEC) {
+        *reinterpret_cast<vec_t*>(row + c) = t;
+    } else if (H > c) {                                  // the end of the row: four, two, one
+        const int left = H - c;
+        T* p = row + c;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e)
-            if (e < left) p[e] = (T)v[e];
+        for (int b = VEC / 2; b > 0; b /= 2)
+            if (left & b) {
+#pragma unroll
+                for (int e = 0; e < VEC / 2; ++e)
+                    if (e < b) p[e] = t[e];
+#pragma unroll
+                for (int e = 0; e + b < VEC; ++e) t[e] = t[e + b];
+                p += b;
+            }
     }
 }
 
+// A row's lanes (LPR: lanes per row, 4 ... 256): up to 64 rows share a workgroup.
+template <int LPR> struct RowShape {
+    static constexpr int WPR = LPR >= 64 ? LPR / 64 : 1, RPW = LPR >= 64 ? 1 : 64 / LPR, RPB = 4 / WPR * RPW;     // waves per row, rows per wave, rows per workgroup
+    static __device__ __forceinline__ int lane() { return LPR >= 64 ? (int)threadIdx.x % LPR : (int)threadIdx.x & (LPR - 1); }
+    static __device__ __forceinline__ int slot() { return (int)threadIdx.x / LPR; }
+};
+
 // sum over the row's WPR waves.  slot: which of the alternating LDS rows this call uses -- a wave may be one call ahead of another, never two.
-template <int WPR>
-__device__ __forceinline__ float row_sum(float s, float (*red)[WPR], int& slot) {
-    s = wave_sum(s);
+template <int LPR>
+__device__ __forceinline__ float row_sum(float s, float (*red)[RowShape<LPR>::WPR], int& slot) {
+    constexpr int WPR = RowShape<LPR>::WPR;
+#pragma unroll
+    for (int o = (LPR < 64 ? LPR : 64) / 2; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
     if constexpr (WPR > 1) {
         const int wave = threadIdx.x >> 6;
         if ((threadIdx.x & 63) == 0) red[slot][wave] = s;
@@ -70,54 +105,54 @@ struct RmsFwdArgs {
     int64_t rows; int H; float eps;
 };
 
-template <typename T, int VEC, int NS, int WPR, bool FULL, bool RES>
+template <typename T, int VEC, int NS, int LPR, bool FULL, bool RES>
 __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwdArgs p) {
-    constexpr int RPB = 4 / WPR;                         // rows in flight per workgroup
-    __shared__ float red[2][WPR];
+    constexpr int RPB = RowShape<LPR>::RPB, SLAB = LPR * VEC;
+    __shared__ float red[2][RowShape<LPR>::WPR];
     int slot = 0;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int c0 = ((wave % WPR) * 64 + lane) * VEC;     // this lane's first feature of a slab
-    constexpr int SLAB = WPR * 64 * VEC;
+    const int c0 = RowShape<LPR>::lane() * VEC;          // this lane's first feature of a slab
     const int H = p.H;
     const T* x = (const T*)p.x;
     const T* res = (const T*)p.res;
-    for (int64_t row = (int64_t)blockIdx.x * RPB + wave / WPR; row < p.rows; row += (int64_t)gridDim.x * RPB) {
+    for (int64_t row = (int64_t)blockIdx.x * RPB + RowShape<LPR>::slot(); row < p.rows; row += (int64_t)gridDim.x * RPB) {
         float v[NS][VEC];
         float ss = 0.f;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             const int c = i * SLAB + c0;
-            load_vec<T, VEC, FULL>(x + row * p.ldx + c, H - c, v[i]);
+            load_vec<T, VEC, FULL, SLAB>(x + row * p.ldx, i * SLAB, c, H, v[i]);
             if constexpr (RES) {
                 float r[VEC];
-                load_vec<T, VEC, FULL>(res + row * p.ldr + c, H - c, r);
+                load_vec<T, VEC, FULL, SLAB>(res + row * p.ldr, i * SLAB, c, H, r);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) v[i][e] = (float)(T)(v[i][e] + r[e]);
-                store_vec<T, VEC, FULL>((T*)p.h + row * H + c, H - c, v[i]);
+                store_vec<T, VEC, FULL, SLAB>((T*)p.h + row * H, i * SLAB, c, H, v[i]);
             }
 #pragma unroll
             for (int e = 0; e < VEC; ++e) ss += v[i][e] * v[i][e];
         }
-        ss = row_sum<WPR>(ss, red, slot);
+        ss = row_sum<LPR>(ss, red, slot);
         const float rstd = 1.0f / sqrtf(ss / (float)H + p.eps);
-        if (p.rstd && lane == 0 && wave % WPR == 0) p.rstd[row] = rstd;
+        if (p.rstd && c0 == 0) p.rstd[row] = rstd;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             const int c = i * SLAB + c0;
             float g[VEC];
-            load_vec<float, VEC, FULL>(p.gamma + c, H - c, g);
+            load_vec<float, VEC, FULL, SLAB>(p.gamma, i * SLAB, c, H, g);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) v[i][e] = v[i][e] * rstd * g[e];
-            if (p.y) store_vec<T, VEC, FULL>((T*)p.y + row * H + c, H - c, v[i]);
-            if (p.y8) {                                  // from the unrounded y: ONE rounding between it and the 8-bit value
-                uint32_t m = 0;
+            if (p.y) store_vec<T, VEC, FULL, SLAB>((T*)p.y + row * H, i * SLAB, c, H, v[i]);
+            if constexpr (SLAB >= 128) {
+                if (p.y8) {                                  // from the unrounded y: ONE rounding between it and the 8-bit value
+                    uint32_t m = 0;
 #pragma unroll
-                for (int e = 0; e < VEC; ++e) m = max(m, __float_as_uint(v[i][e]) & 0x7fffffffu);
-                m = group_umax<128 / VEC>(m);
-                const int byte = block_scale_byte(m, E4M3_TOP);
-                if (FULL || c < p.ld8) {
-                    store_codes<0, VEC>(p.y8 + row * p.ld8 + c, v[i], byte);
-                    if ((c & 127) == 0) p.s8[row * p.lds8 + (c >> 7)] = (uint8_t)byte;
+                    for (int e = 0; e < VEC; ++e) m = max(m, __float_as_uint(v[i][e]) & 0x7fffffffu);
+                    m = group_umax<128 / VEC>(m);
+                    const int byte = block_scale_byte(m, E4M3_TOP);
+                    if (FULL || c < p.ld8) {
+                        store_codes<0, VEC>(p.y8 + row * p.ld8 + c, v[i], byte);
+                        if ((c & 127) == 0) p.s8[row * p.lds8 + (c >> 7)] = (uint8_t)byte;
+                    }
                 }
             }
         }
@@ -134,15 +169,13 @@ struct RmsBwdArgs {
     int64_t rows; int H;
 };
 
-template <typename T, int VEC, int NS, int WPR, bool FULL>
+template <typename T, int VEC, int NS, int LPR, bool FULL>
 __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdArgs p) {
-    constexpr int RPB = 4 / WPR;
-    constexpr int SLAB = WPR * 64 * VEC;
-    __shared__ float red[2][WPR];
+    constexpr int RPB = RowShape<LPR>::RPB, SLAB = LPR * VEC;
+    __shared__ float red[2][RowShape<LPR>::WPR];
     __shared__ float gred[RPB > 1 ? RPB : 1][RPB > 1 ? SLAB : 1];
     int slot = 0;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int c0 = ((wave % WPR) * 64 + lane) * VEC;
+    const int c0 = RowShape<LPR>::lane() * VEC;
     const int H = p.H;
     const T* dy = (const T*)p.dy;
     const T* h = (const T*)p.h;
@@ -152,7 +185,7 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdArgs p) {
     for (int i = 0; i < NS; ++i)
 #pragma unroll
         for (int e = 0; e < VEC; ++e) dg[i][e] = 0.f;
-    for (int64_t row = (int64_t)blockIdx.x * RPB + wave / WPR; row < p.rows; row += (int64_t)gridDim.x * RPB) {
+    for (int64_t row = (int64_t)blockIdx.x * RPB + RowShape<LPR>::slot(); row < p.rows; row += (int64_t)gridDim.x * RPB) {
         const float rs = p.rstd[row];
         float n[NS][VEC], t[NS][VEC];
         float c1 = 0.f;
@@ -160,9 +193,9 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdArgs p) {
         for (int i = 0; i < NS; ++i) {
             const int c = i * SLAB + c0;
             float g[VEC];
-            load_vec<T, VEC, FULL>(h + row * p.ldh + c, H - c, n[i]);
-            load_vec<T, VEC, FULL>(dy + row * p.lddy + c, H - c, t[i]);
-            load_vec<float, VEC, FULL>(p.gamma + c, H - c, g);
+            load_vec<T, VEC, FULL, SLAB>(h + row * p.ldh, i * SLAB, c, H, n[i]);
+            load_vec<T, VEC, FULL, SLAB>(dy + row * p.lddy, i * SLAB, c, H, t[i]);
+            load_vec<float, VEC, FULL, SLAB>(p.gamma, i * SLAB, c, H, g);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
                 n[i][e] *= rs;
@@ -171,7 +204,7 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdArgs p) {
                 c1 += t[i][e] * n[i][e];
             }
         }
-        c1 = row_sum<WPR>(c1, red, slot) / (float)H;
+        c1 = row_sum<LPR>(c1, red, slot) / (float)H;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             const int c = i * SLAB + c0;
@@ -180,11 +213,11 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdArgs p) {
             for (int e = 0; e < VEC; ++e) o[e] = rs * (t[i][e] - n[i][e] * c1);
             if (dres) {
                 float r[VEC];
-                load_vec<T, VEC, FULL>(dres + row * p.lddr + c, H - c, r);
+                load_vec<T, VEC, FULL, SLAB>(dres + row * p.lddr, i * SLAB, c, H, r);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) o[e] += r[e];
             }
-            store_vec<T, VEC, FULL>((T*)p.dx + row * H + c, H - c, o);
+            store_vec<T, VEC, FULL, SLAB>((T*)p.dx + row * H, i * SLAB, c, H, o);
         }
     }
     // the workgroup's rows together, in a fixed order; the partial sums are added up by rms_dgamma_kernel (no atomics: the same call gives the same bits)
@@ -194,7 +227,7 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdArgs p) {
         if constexpr (RPB > 1) {
             __syncthreads();
 #pragma unroll
-            for (int e = 0; e < VEC; ++e) gred[wave][lane * VEC + e] = dg[i][e];
+            for (int e = 0; e < VEC; ++e) gred[RowShape<LPR>::slot()][c0 + e] = dg[i][e];
             __syncthreads();
             for (int k = threadIdx.x; k < SLAB; k += 256)
                 if (i * SLAB + k < H) {
@@ -204,7 +237,7 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdArgs p) {
                     p.part[(int64_t)blockIdx.x * H + i * SLAB + k] = s;
                 }
         } else {
-            store_vec<float, VEC, FULL>(p.part + (int64_t)blockIdx.x * H + c, H - c, dg[i]);
+            store_vec<float, VEC, FULL, SLAB>(p.part + (int64_t)blockIdx.x * H, i * SLAB, c, H, dg[i]);
         }
     }
 }
@@ -229,42 +262,48 @@ __global__ __launch_bounds__(1024) void rms_dgamma_kernel(const float* __restric
 
 constexpr int RMS_MAX_H = 16384;
 
-// (VEC, NS, WPR) by width: one wave and 8 features per lane up to 2 048, but 4 per lane where 8 would leave half of the last slab's lanes idle (ceil(H / 256)
-// odd, up to 768); four waves above
-#define RMS_WIDTH(H, V, N, W, ...)                                                                             \
+// (VEC, slabs, lanes per row) by width.  8 features per lane, 4 where 8 would leave half of the last slab's lanes idle (up to 256 and 768); several rows per wave up to 128
+// (200000 x 64 bf16, a wave per row : eight rows: RMS_NARROW), four waves per row above 2 048.  narrow: not with the 8-bit copy, whose blocks of 128 are a row's own sixteen lanes
+#define RMS_WIDTH(H, V, N, L, ...)                                                                             \
     do {                                                                                                        \
-        constexpr int VEC = V, NS = N, WPR = W;                                                                 \
-        if ((H) == VEC * 64 * WPR * NS) { constexpr bool FULL = true; __VA_ARGS__; }                                   \
+        constexpr int VEC = V, NS = N, LPR = L;                                                                 \
+        if ((H) == VEC * LPR * NS) { constexpr bool FULL = true; __VA_ARGS__; }                                        \
         else { constexpr bool FULL = false; __VA_ARGS__; }                                                             \
     } while (0)
-#define RMS_DISPATCH(H, ...)                                                                                   \
+#define RMS_DISPATCH(H, narrow, ...)                                                                           \
     do {                                                                                                        \
-        if ((H) <= 256) RMS_WIDTH(H, 4, 1, 1, __VA_ARGS__);                                                            \
-        else if ((H) <= 512) RMS_WIDTH(H, 8, 1, 1, __VA_ARGS__);                                                       \
-        else if ((H) <= 768) RMS_WIDTH(H, 4, 3, 1, __VA_ARGS__);                                                       \
-        else if ((H) <= 1024) RMS_WIDTH(H, 8, 2, 1, __VA_ARGS__);                                                      \
-        else if ((H) <= 2048) RMS_WIDTH(H, 8, 4, 1, __VA_ARGS__);                                                      \
-        else if ((H) <= 4096) RMS_WIDTH(H, 8, 2, 4, __VA_ARGS__);                                                      \
-        else if ((H) <= 8192) RMS_WIDTH(H, 8, 4, 4, __VA_ARGS__);                                                      \
-        else RMS_WIDTH(H, 8, 8, 4, __VA_ARGS__);                                                                       \
+        if ((H) <= 32 && (narrow)) RMS_WIDTH(H, 8, 1, 4, __VA_ARGS__);                                                 \
+        else if ((H) <= 64 && (narrow)) RMS_WIDTH(H, 8, 1, 8, __VA_ARGS__);                                            \
+        else if ((H) <= 128) RMS_WIDTH(H, 8, 1, 16, __VA_ARGS__);                                                      \
+        else if ((H) <= 256) RMS_WIDTH(H, 4, 1, 64, __VA_ARGS__);                                                      \
+        else if ((H) <= 512) RMS_WIDTH(H, 8, 1, 64, __VA_ARGS__);                                                      \
+        else if ((H) <= 768) RMS_WIDTH(H, 4, 3, 64, __VA_ARGS__);                                                      \
+        else if ((H) <= 1024) RMS_WIDTH(H, 8, 2, 64, __VA_ARGS__);                                                     \
+        else if ((H) <= 1536) RMS_WIDTH(H, 8, 3, 64, __VA_ARGS__);                                                     \
+        else if ((H) <= 2048) RMS_WIDTH(H, 8, 4, 64, __VA_ARGS__);                                                     \
+        else if ((H) <= 4096) RMS_WIDTH(H, 8, 2, 256, __VA_ARGS__);                                                    \
+        else if ((H) <= 6144) RMS_WIDTH(H, 8, 3, 256, __VA_ARGS__);                                                    \
+        else if ((H) <= 8192) RMS_WIDTH(H, 8, 4, 256, __VA_ARGS__);                                                    \
+        else RMS_WIDTH(H, 8, 8, 256, __VA_ARGS__);                                                                     \
     } while (0)
 
-int rms_rows_per_block(int H) { return H <= 2048 ? 4 : 1; }
+int rms_rows_per_block(int H, bool narrow) { return H <= 32 && narrow ? 64 : H <= 64 && narrow ? 32 : H <= 128 ? 16 : H <= 2048 ? 4 : 1; }
 
 // 1 024 workgroups: 101376 x 768 takes 160 us with 512, 121 with 1 024, 134 with 2 048 (more partial rows to write and add up)
 int rms_bwd_blocks(int64_t rows, int H) {
-    const int64_t nb = (rows + rms_rows_per_block(H) - 1) / rms_rows_per_block(H);
+    const int64_t rpb = rms_rows_per_block(H, true), nb = (rows + rpb - 1) / rpb;
     return (int)(nb < 1024 ? nb : 1024);
 }
 
 template <typename T>
 void rms_fwd_launch(const RmsFwdArgs& a, hipStream_t s) {
-    const int64_t nb = (a.rows + rms_rows_per_block(a.H) - 1) / rms_rows_per_block(a.H);
+    const bool narrow = !a.y8;
+    const int64_t rpb = rms_rows_per_block(a.H, narrow), nb = (a.rows + rpb - 1) / rpb;
     const dim3 grid((unsigned)(nb < 4096 ? nb : 4096)), block(256);
     if (a.res)
-        RMS_DISPATCH(a.H, hipLaunchKernelGGL((rms_fwd_kernel<T, VEC, NS, WPR, FULL, true>), grid, block, 0, s, a));
+        RMS_DISPATCH(a.H, narrow, hipLaunchKernelGGL((rms_fwd_kernel<T, VEC, NS, LPR, FULL, true>), grid, block, 0, s, a));
     else
-        RMS_DISPATCH(a.H, hipLaunchKernelGGL((rms_fwd_kernel<T, VEC, NS, WPR, FULL, false>), grid, block, 0, s, a));
+        RMS_DISPATCH(a.H, narrow, hipLaunchKernelGGL((rms_fwd_kernel<T, VEC, NS, LPR, FULL, false>), grid, block, 0, s, a));
 }
 
 }  // namespace
@@ -301,8 +340,8 @@ extern "C" int merlot_rms_bwd(const void* dy, int64_t lddy, int is_f32, const vo
     const RmsBwdArgs a = {dy, lddy, h, ldh, rstd, gamma, dres, lddr, dx, (float*)workspace, rows, H};
     hipStream_t s = (hipStream_t)stream;
     const dim3 grid(nb), block(256);
-    if (is_f32) RMS_DISPATCH(H, hipLaunchKernelGGL((rms_bwd_kernel<float, VEC, NS, WPR, FULL>), grid, block, 0, s, a));
-    else RMS_DISPATCH(H, hipLaunchKernelGGL((rms_bwd_kernel<bf16, VEC, NS, WPR, FULL>), grid, block, 0, s, a));
+    if (is_f32) RMS_DISPATCH(H, true, hipLaunchKernelGGL((rms_bwd_kernel<float, VEC, NS, LPR, FULL>), grid, block, 0, s, a));
+    else RMS_DISPATCH(H, true, hipLaunchKernelGGL((rms_bwd_kernel<bf16, VEC, NS, LPR, FULL>), grid, block, 0, s, a));
     if (int rc = merlot_launch_status("merlot_rms_bwd")) return rc;
     hipLaunchKernelGGL(rms_dgamma_kernel, dim3((H + 63) / 64), dim3(1024), 0, s, (const float*)workspace, dgamma, nb, H);
     return merlot_launch_status("merlot_rms_bwd");

@@ -35,8 +35,9 @@ def _close(got, want, tol, what):
     assert not bool(bad.any()), (what, int(bad.sum()), float(((got.double().cpu() - want).abs() / tol.clamp(min=1e-300)).max()))
 
 
-# every (elements per lane, slabs, waves per row) variant, its first and last width, odd widths, and views whose rows are 2- or 4-byte aligned only
-WIDTHS = [1, 7, 8, 127, 128, 130, 255, 256, 257, 500, 512, 768, 769, 1000, 1001, 1024, 2047, 2048, 2049, 4096, 4100, 8192, 8200, 16384]
+# every (elements per lane, slabs, lanes per row) variant, its first and last width, odd widths, and views whose rows are 2- or 4-byte aligned only
+WIDTHS = [1, 2, 7, 8, 9, 16, 31, 32, 33, 63, 64, 65, 100, 127, 128, 130, 255, 256, 257, 500, 512, 768, 769, 1000, 1001, 1024, 1025, 1531, 1536, 1537, 2047, 2048, 2049, 4096, 4100, 5001,
+          6144, 6145, 8192, 8200, 16384]
 
 
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
@@ -57,6 +58,10 @@ def test_forward_and_backward(H, dtype):
         steps = (H / 64 + 16) / 2 + 6
         _close(y, yr, yr.abs() * (steps * U + HALF[dtype]) + 1e-40, 'y')
         _close(rstd, rr[:, 0], rr[:, 0] * steps * U, 'rstd')
+        alone = ops.rms_norm_fwd(xg, gamma.cuda(), residual=None if res is None else res.cuda(), eps=EPS)      # narrow rows: fewer lanes each without the 8-bit copy
+        _close(alone[0], yr, yr.abs() * (steps * U + HALF[dtype]) + 1e-40, 'y alone')
+        _close(alone[2], rr[:, 0], rr[:, 0] * steps * U, 'rstd alone')
+        assert h is None or torch.equal(alone[1], h)
         # the 8-bit copy of the unrounded y: half a step of e4m3 (2^-4 of the value, or of the least normal 2^-6 of the block's unit) beside y's own error; a block whose
         # maximum lies within y's error of a border of the scale may take the neighbouring power of two, whose half steps are twice as large only below the normal range
         _, _, v = ref.quantize(yr, 0)
