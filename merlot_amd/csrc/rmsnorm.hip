@@ -3,9 +3,10 @@
 //   h = round(x + residual);  R = 1 / sqrt(mean(h^2) + eps);  y = h * R * gamma
 //   n = h * R;  t = dy * gamma;  dx = R * (t - n * mean(t * n)) (+ dres);  dgamma += sum over rows of dy * n
 //
-// Both directions are bound by memory: every operand crosses it once.  A row is held in registers by WPR waves (1 up to 2 048 features, 4 above), each lane
-// VEC consecutive features per slab, so a lane's loads and stores are 8 or 16 bytes and the 128 features that share a scale lie in 128 / VEC neighbouring lanes.
-// Measured (101376 x 768 bf16): forward with residual 114 us = 5.45 TB/s (a large copy: 4.85 TB/s), with the 8-bit copy in place of y 103 us, backward with
+// Both directions are bound by memory: every operand crosses it once.  A row is held in registers by 4 ... 64 lanes of a wave (up to 2 048 features) or by
+// four waves, each lane VEC consecutive features per slab, so a lane's loads and stores are 8 or 16 bytes and the 128 features that share a scale lie in 128 / VEC
+// neighbouring lanes.
+// Measured (101376 x 768 bf16): forward with residual 117 us = 5.3 TB/s (a large copy: 4.85 TB/s), with the 8-bit copy in place of y 103 us, backward with
 // the residual stream's gradient 120 us + 5 us for dgamma = 5.0 TB/s.  Widths that are whole slabs take code without per-element branches (FULL: backward 184 -> 120 us).
 // All sums are fp32.  The statistics are taken from h AS STORED (rounded to its type), so that the backward, which reads the stored h, differentiates the
 // function the forward computed.
@@ -17,33 +18,48 @@ namespace {
 // VEC consecutive elements at any element alignment (gfx950 loads and stores global dwords at byte alignment): rows of odd width need no path of their own
 template <typename T, int VEC> struct ElemVec { typedef T type __attribute__((ext_vector_type(VEC), aligned(sizeof(T)))); };
 
-// elements c ... c + VEC - 1 of a row of H; those past its end are zeros and are not stored.  FULL: H is a whole number of slabs.  base: the slab's first element, the same
-// in every lane -- whole slabs take no checks.  In the slab that the row's end lies in every lane loads one vector all the same, the lane at the end the row's last VEC elements,
-// which it moves down (50000 x 2000 bf16: element by element the backward took 267 us, this way RMS_ODD).
+// Elements c ... c + VEC - 1 of a row of H; those past its end are zeros and are not stored.  FULL: H is a whole number of slabs.  base: the slab's first element, the same
+// in every lane.  In the slab that the row's end lies in the lane at the end loads the row's last VEC elements and moves them down, and
+// a row's loads come before all conversions, so that they are in flight together (element by element, 100000 x 500 bf16 backward: 177 us, this way 89).
 template <typename T, int VEC, bool FULL, int SLAB>
-__device__ __forceinline__ void load_vec(const T* row, int base, int c, int H, float (&v)[VEC]) {
+__device__ __forceinline__ void load_raw(const T* row, int base, int c, int H, typename ElemVec<T, VEC>::type& t) {
     typedef typename ElemVec<T, VEC>::type vec_t;
-    if (FULL || base + SLAB <= H) {
-        const vec_t t = *reinterpret_cast<const vec_t*>(row + c);
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = (float)t[e];
-    } else if (base >= H) {
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = 0.f;
-    } else if (H >= VEC) {
-        const int left = H - c;
-        const vec_t t = *reinterpret_cast<const vec_t*>(row + (left >= VEC ? c : left > 0 ? H - VEC : 0));
-        const int s = left >= VEC ? 0 : VEC - left;
-#pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = left > 0 ? (float)t[e] : 0.f;
-#pragma unroll
-        for (int b = 1; b < VEC; b *= 2)
-#pragma unroll
-            for (int e = 0; e < VEC; ++e) v[e] = left > 0 && (s & b) ? (e + b < VEC ? v[e + b] : 0.f) : v[e];
+    if (FULL) {
+        t = *reinterpret_cast<const vec_t*>(row + c);
+    } else if (SLAB > 128 && base < H && H >= VEC) {     // lanes behind the end read the row's start: a branch around the load would wait for what is in flight (50000 x 2000
+        t = *reinterpret_cast<const vec_t*>(row + (H - c >= VEC ? c : c < H ? H - VEC : 0));     // bf16 backward 250 us, without 165), but pays in narrow rows (x 8: 9.6 us, with 7.7)
     } else {
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) v[e] = c + e < H ? (float)row[c + e] : 0.f;
+        for (int e = 0; e < VEC; ++e) t[e] = (T)0.f;
+        if (H >= VEC) {
+            if (c < H) t = *reinterpret_cast<const vec_t*>(row + min(c, H - VEC));
+        } else {                                         // a row shorter than a vector
+#pragma unroll
+            for (int e = 0; e < VEC; ++e)
+                if (c + e < H) t[e] = row[c + e];
+        }
     }
+}
+template <typename T, int VEC, bool FULL, int SLAB>
+__device__ __forceinline__ void expand(const typename ElemVec<T, VEC>::type& t, int base, int c, int H, float (&v)[VEC]) {
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = (float)t[e];
+    if (FULL || base + SLAB <= H || H < VEC) return;
+#pragma unroll
+    for (int e = 0; e < VEC; ++e) v[e] = c < H ? v[e] : 0.f;
+    const int s = -H & (VEC - 1);                        // by how much: the same in every row
+    const bool end = c < H && H - c < VEC;
+#pragma unroll
+    for (int b = 1; b < VEC; b *= 2)
+        if (s & b)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) v[e] = end ? (e + b < VEC ? v[e + b] : 0.f) : v[e];
+}
+template <typename T, int VEC, bool FULL, int SLAB>
+__device__ __forceinline__ void load_vec(const T* row, int base, int c, int H, float (&v)[VEC]) {
+    typename ElemVec<T, VEC>::type t;
+    load_raw<T, VEC, FULL, SLAB>(row, base, c, H, t);
+    expand<T, VEC, FULL, SLAB>(t, base, c, H, v);
 }
 template <typename T, int VEC, bool FULL, int SLAB>
 __device__ __forceinline__ void store_vec(T* row, int base, int c, int H, const float (&v)[VEC]) {
@@ -117,13 +133,19 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwdArgs p) {
     for (int64_t row = (int64_t)blockIdx.x * RPB + RowShape<LPR>::slot(); row < p.rows; row += (int64_t)gridDim.x * RPB) {
         float v[NS][VEC];
         float ss = 0.f;
+        typename ElemVec<T, VEC>::type tx[NS], tr[NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            load_raw<T, VEC, FULL, SLAB>(x + row * p.ldx, i * SLAB, i * SLAB + c0, H, tx[i]);
+            if constexpr (RES) load_raw<T, VEC, FULL, SLAB>(res + row * p.ldr, i * SLAB, i * SLAB + c0, H, tr[i]);
+        }
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             const int c = i * SLAB + c0;
-            load_vec<T, VEC, FULL, SLAB>(x + row * p.ldx, i * SLAB, c, H, v[i]);
+            expand<T, VEC, FULL, SLAB>(tx[i], i * SLAB, c, H, v[i]);
             if constexpr (RES) {
                 float r[VEC];
-                load_vec<T, VEC, FULL, SLAB>(res + row * p.ldr, i * SLAB, c, H, r);
+                expand<T, VEC, FULL, SLAB>(tr[i], i * SLAB, c, H, r);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) v[i][e] = (float)(T)(v[i][e] + r[e]);
                 store_vec<T, VEC, FULL, SLAB>((T*)p.h + row * H, i * SLAB, c, H, v[i]);
@@ -171,6 +193,9 @@ struct RmsBwdArgs {
 
 template <typename T, int VEC, int NS, int LPR, bool FULL>
 __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdArgs p) {
+    // dres is asked for with the other operands where a lane holds much of a row (few waves fit a CU); with less the registers cost more waves than it gains (us, late : early,
+    // bf16: 20000 x 5000 222 : 169, 50000 x 2000 182 : 165, 10000 x 8192 150 : 136; 20000 x 4096 126 : 139, 101376 x 768 122 : 128)
+    constexpr bool EARLY = NS * VEC >= 24;
     constexpr int RPB = RowShape<LPR>::RPB, SLAB = LPR * VEC;
     __shared__ float red[2][RowShape<LPR>::WPR];
     __shared__ float gred[RPB > 1 ? RPB : 1][RPB > 1 ? SLAB : 1];
@@ -189,12 +214,19 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdArgs p) {
         const float rs = p.rstd[row];
         float n[NS][VEC], t[NS][VEC];
         float c1 = 0.f;
+        typename ElemVec<T, VEC>::type th[NS], td[NS], te[NS];
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            load_raw<T, VEC, FULL, SLAB>(h + row * p.ldh, i * SLAB, i * SLAB + c0, H, th[i]);
+            load_raw<T, VEC, FULL, SLAB>(dy + row * p.lddy, i * SLAB, i * SLAB + c0, H, td[i]);
+            if (EARLY && dres) load_raw<T, VEC, FULL, SLAB>(dres + row * p.lddr, i * SLAB, i * SLAB + c0, H, te[i]);
+        }
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             const int c = i * SLAB + c0;
             float g[VEC];
-            load_vec<T, VEC, FULL, SLAB>(h + row * p.ldh, i * SLAB, c, H, n[i]);
-            load_vec<T, VEC, FULL, SLAB>(dy + row * p.lddy, i * SLAB, c, H, t[i]);
+            expand<T, VEC, FULL, SLAB>(th[i], i * SLAB, c, H, n[i]);
+            expand<T, VEC, FULL, SLAB>(td[i], i * SLAB, c, H, t[i]);
             load_vec<float, VEC, FULL, SLAB>(p.gamma, i * SLAB, c, H, g);
 #pragma unroll
             for (int e = 0; e < VEC; ++e) {
@@ -213,7 +245,8 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdArgs p) {
             for (int e = 0; e < VEC; ++e) o[e] = rs * (t[i][e] - n[i][e] * c1);
             if (dres) {
                 float r[VEC];
-                load_vec<T, VEC, FULL, SLAB>(dres + row * p.lddr, i * SLAB, c, H, r);
+                if (!EARLY) load_raw<T, VEC, FULL, SLAB>(dres + row * p.lddr, i * SLAB, c, H, te[i]);
+                expand<T, VEC, FULL, SLAB>(te[i], i * SLAB, c, H, r);
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) o[e] += r[e];
             }
@@ -263,7 +296,7 @@ __global__ __launch_bounds__(1024) void rms_dgamma_kernel(const float* __restric
 constexpr int RMS_MAX_H = 16384;
 
 // (VEC, slabs, lanes per row) by width.  8 features per lane, 4 where 8 would leave half of the last slab's lanes idle (up to 256 and 768); several rows per wave up to 128
-// (200000 x 64 bf16, a wave per row : eight rows: RMS_NARROW), four waves per row above 2 048.  narrow: not with the 8-bit copy, whose blocks of 128 are a row's own sixteen lanes
+// (200000 x 64 bf16, a wave per row : eight rows: forward 51 : 17 us, backward 84 : 21), four waves per row above 2 048.  narrow: not with the 8-bit copy, whose blocks of 128 are a row's own sixteen lanes
 #define RMS_WIDTH(H, V, N, L, ...)                                                                             \
     do {                                                                                                        \
         constexpr int VEC = V, NS = N, LPR = L;                                                                 \
