@@ -739,31 +739,34 @@ struct BlocksPlan { int bm, bn, splits, nk_split; };
 // With rows of C that start inside a 64-byte sector their 128-byte row pieces are written as parts of lines, past the caches or not: 101376 x 2296 x 768 225 : 306, and only a
 // long reduction hides it (30000 x 2296 x 2048 163 : 147, x 4096 297 : 254; 4099 x 50370 x 2048 467 : 476).
 // fp32 outputs with such rows: 16384 x 4096 x 256 70 : 67, x 768 118 : 112; 8192^3 870 : 787; 4099 x 50304 x 768 344 : 322; with others not (4099 x 50370 x 768 374 : 458).  Added
-// onto what is there they stay with 128 x 256 (the wide epilogue has no time to wait for old values).  Their long reductions are split over 256 x 256 tiles where each workgroup gets
-// enough of them (128-row tiles, split as below : 256 x 256): 4096 x 1024 x 32768 238 : 209, 2304 x 768 x 101376 330 : 286, x 12544 62 : 59, 1024 x 1024 x 16384 58 : 52,
-// 2304 x 2304 x 8192 108 : 93; but where narrow tiles need no split, 2304 x 2304 x 4096, 55 : 61.
+// onto what is there they stay with 128 x 256 (the wide epilogue has no time to wait for old values).  Their long reductions are split over 256 x 256 tiles, at least half of which is
+// the product's, where a workgroup gets ten blocks, or 18 if narrow tiles need no split (split over narrow tiles : 256 x 256): 4096 x 1024 x 32768 235 : 209, 2304 x 768 x 101376
+// 325 : 288, x 12544 65 : 60, 2304 x 2304 x 8192 99 : 92; but 1024 x 1024 x 16384 46 : 52, 1000 x 4096 x 4096 43 : 55, 64 x 8192 x 8192 28 : 39.
 // 128 x 256 where those fill the CUs twice; otherwise the reduction is split, or narrow tiles.
 BlocksPlan blocks_plan(int64_t M, int64_t N, int64_t K, bool out_bf16, bool accumulate, bool whole_lines) {
     const int64_t tm = (M + 127) / 128, nk = K / 128;
     // straight from memory: 16 x 16, 32 x 16 or 64 x 32 outputs per workgroup
     const int mf = M <= 16 ? 1 : M <= 32 ? 2 : 4, nf = mf == 4 ? 2 : 1;
     if (nk <= 8 * direct_unroll(mf) * (mf == 1 ? 2 : 1) && (M + 16 * mf - 1) / (16 * mf) * ((N + 16 * nf - 1) / (16 * nf)) * (mf + nf) <= 3000) return {16 * mf, 16 * nf, 1, (int)nk};
-    if (out_bf16 && nk >= (whole_lines ? 4 : 16) && ((M + 255) / 256) * ((N + 255) / 256) >= 256) return {256, 256, 1, (int)nk};
-    const int64_t tw = ((M + 255) / 256) * ((N + 255) / 256);
+    const int64_t tw = ((M + 255) / 256) * ((N + 255) / 256), wide = tm * ((N + 255) / 256), narrow = tm * ((N + 127) / 128);     // tiles of 256 x 256, 128 x 256, 128 x 128
+    if (out_bf16 && nk >= (whole_lines ? 4 : 16) && tw >= 256) return {256, 256, 1, (int)nk};
     if (!out_bf16 && !accumulate && whole_lines && nk >= 2 && tw >= 256) return {256, 256, 1, (int)nk};
-    if (!out_bf16 && N > 128 && tw <= 128 && nk * tw / 256 >= (tw > 64 ? 16 : 8)) {
+    if (!out_bf16 && tw <= 128 && 2 * M * N >= tw * 65536 && nk * tw / 256 >= (narrow > 128 ? 18 : 10)) {
         const int64_t s = 256 / tw, per = ((nk + s - 1) / s + 3) / 4 * 4;
         if ((nk + per - 1) / per > 1) return {256, 256, (int)((nk + per - 1) / per), (int)per};
     }
-    if (N > 128 && tm * ((N + 255) / 256) >= 512) return {128, 256, 1, (int)nk};
-    // a long reduction: split until there are about 512 workgroups, 24 blocks each at least with the wide tile, eight with the narrow one (fp32, narrow : wide:
-    // 4096 x 1024 x 32768 251 : 236, 2304 x 768 x 101376 370 : 328; but 18 wide tiles, 768 x 768 x 65536, 92 : 102)
-    for (int bn = N > 128 ? 256 : 128; bn >= 128; bn -= 128) {
-        const int64_t tiles = tm * ((N + bn - 1) / bn), s = min(512 / tiles, nk / (bn == 256 ? 24 : 8));
-        if (s < 2 || (bn == 256 && tiles < 32)) continue;
+    if (N > 128 && wide >= 512) return {128, 256, 1, (int)nk};
+    // long reductions are split: 128 x 256 tiles over three quarters of both places of every CU at least, where each workgroup keeps 24 blocks (us, bf16, narrow tiles in 7 parts : this way:
+    // 2304 x 768 x 101376 280 : 238, x 24576 76 : 68; with 378 workgroups, 768 x 768 x 65536, 67 : 83); otherwise narrow tiles over one place of every CU, six blocks each at least (a
+    // second workgroup on a CU gains 8 % of the time per block and costs another set of partial products: 1024 x 1024 x 8192, 64 tiles, in 4 : 8 parts 22 : 27, 256 x 4096 x 4096
+    // 18 : 22).  Up to 16 blocks the second launch costs more than it saves (1024 x 1024 x 2048 whole 13, in two 15; 2000 x 1000 x 2048 14 : 19).
+    auto parts = [&](int bn, int64_t s) -> BlocksPlan {
         const int64_t per = ((nk + s - 1) / s + 3) / 4 * 4;
         return {128, bn, (int)((nk + per - 1) / per), (int)per};
-    }
+    };
+    const int64_t sw = min(512 / wide, nk / 24), sn = min(256 / narrow, nk / 6);
+    if (N > 128 && narrow <= 256 && sw >= 2 && wide * sw >= 384) return parts(256, sw);
+    if (nk > 16 && sn >= 2) return parts(128, sn);
     return {128, 128, 1, (int)nk};
 }
 

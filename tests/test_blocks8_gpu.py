@@ -149,7 +149,8 @@ def _whole_on_device(rows, K, fmt, seed):
 # blocks, more tiles than workgroups; 128 x 256 tiles: short K, fp32 onto what is there, odd N; split reductions with tiles of 128, 256 columns and 256 x 256 (N = 1030: partial
 # products with padded rows, a last split of one block)
 @pytest.mark.parametrize('M,N,K', [(4096, 4096, 512), (8200, 2080, 640), (4100, 4384, 2304), (4200, 4300, 2176), (20000, 1120, 768), (33000, 512, 256), (33000, 500, 384), (2304, 768, 6272),
-                                   (300, 200, 9216), (16500, 1028, 128), (2304, 768, 12544), (1100, 1030, 16512), (500, 300, 65664)])
+                                   (300, 200, 9216), (16500, 1028, 128), (2304, 768, 12544), (1100, 1030, 16512), (500, 300, 65664), (2304, 768, 24576),
+                                   (4224, 260, 18432), (700, 700, 2944)])
 @pytest.mark.parametrize('fa', [0, 1])
 def test_large_products_of_whole_numbers_are_exact(M, N, K, fa):
     """sum |a b| < 2^24 (asserted): exact in fp32 in any order, in every kernel; the fp32 reference product is exact for the same reason"""
