@@ -7,7 +7,7 @@
 // four waves, each lane VEC consecutive features per slab, so a lane's loads and stores are 8 or 16 bytes and the 128 features that share a scale lie in 128 / VEC
 // neighbouring lanes.
 // Measured (101376 x 768 bf16): forward with residual 117 us = 5.3 TB/s (a large copy: 4.85 TB/s), with the 8-bit copy in place of y 103 us, backward with
-// the residual stream's gradient 120 us + 5 us for dgamma = 5.0 TB/s.  Widths that are whole slabs take code without per-element branches (FULL: backward 184 -> 120 us).
+// the residual stream's gradient 122 us with dgamma = 5.1 TB/s.  Widths that are whole slabs take code without per-element branches (FULL: backward 184 -> 120 us).
 // All sums are fp32.  The statistics are taken from h AS STORED (rounded to its type), so that the backward, which reads the stored h, differentiates the
 // function the forward computed.
 #include "common.h"
@@ -275,20 +275,25 @@ __global__ __launch_bounds__(256) void rms_bwd_kernel(const RmsBwdArgs p) {
     }
 }
 
-// dgamma[c] += sum over the nb partial rows, 64 columns x 16 row groups per workgroup
+// dgamma[c] += sum over the nb partial rows, COLS columns x 1024 / COLS row groups per workgroup: 16 up to 2 048 features, so that enough CUs take part, 64 above (whole backward, 64 : 16
+// columns: 8000 x 768 16.1 : 15.2 us, 4099 x 1001 18.8 : 17.4; 8192 x 8192 112 : 116)
+template <int COLS>
 __global__ __launch_bounds__(1024) void rms_dgamma_kernel(const float* __restrict__ part, float* __restrict__ dgamma, int nb, int H) {
-    __shared__ float red[16][64];
-    const int col = blockIdx.x * 64 + (threadIdx.x & 63), grp = threadIdx.x >> 6;
+    __shared__ float red[16][COLS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, c = threadIdx.x % COLS, col = blockIdx.x * COLS + c;
     float s = 0.f;
     if (col < H) {
 #pragma unroll 8
-        for (int r = grp; r < nb; r += 16) s += part[(int64_t)r * H + col];
+        for (int r = threadIdx.x / COLS; r < nb; r += 1024 / COLS) s += part[(int64_t)r * H + col];
     }
-    red[grp][threadIdx.x & 63] = s;
-    __syncthreads();
-    if (grp == 0 && col < H) {
 #pragma unroll
-        for (int w = 1; w < 16; ++w) s += red[w][threadIdx.x];
+    for (int o = COLS; o < 64; o *= 2) s += __shfl_xor(s, o, 64);
+    if (lane < COLS) red[wave][c] = s;
+    __syncthreads();
+    if (threadIdx.x < COLS && col < H) {
+        s = red[0][c];
+#pragma unroll
+        for (int w = 1; w < 16; ++w) s += red[w][c];
         dgamma[col] += s;
     }
 }
@@ -376,6 +381,7 @@ extern "C" int merlot_rms_bwd(const void* dy, int64_t lddy, int is_f32, const vo
     if (is_f32) RMS_DISPATCH(H, true, hipLaunchKernelGGL((rms_bwd_kernel<float, VEC, NS, LPR, FULL>), grid, block, 0, s, a));
     else RMS_DISPATCH(H, true, hipLaunchKernelGGL((rms_bwd_kernel<bf16, VEC, NS, LPR, FULL>), grid, block, 0, s, a));
     if (int rc = merlot_launch_status("merlot_rms_bwd")) return rc;
-    hipLaunchKernelGGL(rms_dgamma_kernel, dim3((H + 63) / 64), dim3(1024), 0, s, (const float*)workspace, dgamma, nb, H);
+    if (H <= 2048) hipLaunchKernelGGL(rms_dgamma_kernel<16>, dim3((H + 15) / 16), dim3(1024), 0, s, (const float*)workspace, dgamma, nb, H);
+    else hipLaunchKernelGGL(rms_dgamma_kernel<64>, dim3((H + 63) / 64), dim3(1024), 0, s, (const float*)workspace, dgamma, nb, H);
     return merlot_launch_status("merlot_rms_bwd");
 }
