@@ -951,8 +951,13 @@ def _dense(t, n, dev, name):
 def _scales8(rows, cols, like):
     """scale bytes of `rows` rows of `cols` values, a byte per block of 128; rows 4-byte aligned (the product reads them as words)"""
     nb = (cols + 127) // 128
-    s = like.new_empty((rows, (nb + 3) // 4 * 4), dtype=torch.uint8)
-    return s if nb % 4 == 0 else s[:, :nb]
+    ld = (nb + 3) // 4 * 4
+    s = like.new_empty((rows, ld), dtype=torch.uint8)
+    return s if nb == ld else s.as_strided((rows, nb), (ld, 1))
+
+
+def _dense_like(x):
+    return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)     # (the first takes 1.2 us, the second 1.7)
 
 
 def rms_norm_fwd(x, gamma, *, residual=None, out=True, q8=False, save_rstd=True, eps=1e-6):
@@ -976,8 +981,8 @@ def rms_norm_fwd(x, gamma, *, residual=None, out=True, q8=False, save_rstd=True,
         if residual.shape != shape:
             raise ValueError(f"residual: expected {tuple(shape)}, got {tuple(residual.shape)}")
         ldr = _rows(residual, dt, dev, 'residual')[2]
-        h = x.new_empty(shape)
-    y = x.new_empty(shape) if out else None
+        h = _dense_like(x)
+    y = _dense_like(x) if out else None
     rstd = gamma.new_empty(rows) if save_rstd else None
     y8 = s8 = None
     if q8:
@@ -1006,7 +1011,7 @@ def rms_norm_bwd(dy, h, rstd, gamma, dgamma, *, dres=None):
     _dense(gamma, H, dev, 'gamma')
     _dense(dgamma, H, dev, 'dgamma')
     _dense(rstd, rows, dev, 'rstd')
-    dx = h.new_empty(shape)
+    dx = _dense_like(h)
     if rows:
         nbytes = LIB.query('merlot_rms_bwd_workspace_bytes', rows, H)
         ws = gamma.new_empty(nbytes // 4)
