@@ -550,7 +550,8 @@ int64_t merlot_example_index(const void* buf, int64_t n, int64_t* rows, int64_t 
  * added entries, so the ABI version stands.
  * ---------------------------------------------------------------------------------------------- */
 /* h = round(x + residual), R = 1 / sqrt(mean(h^2) + eps), y = h * R * gamma over rows of H features, any H from 1 to 16 384; statistics fp32, taken from h
- * AS STORED.  x, residual, h, y all bf16 (x_f32 0) or all f32; x and residual with row strides ldx / ldr >= H, h and y dense.  residual and h: both or neither
+ * AS STORED; a finite row has its y whatever its magnitude (the squares may leave fp32).  Where R itself is no normal fp32 number -- mean(h^2) over 2^252: it keeps 21
+ * bits; mean(h^2) + eps under 2^-256: it is infinite -- y does not suffer, the backward's n = h * R does.  x, residual, h, y all bf16 (x_f32 0) or all f32; x and residual with row strides ldx / ldr >= H, h and y dense.  residual and h: both or neither
  * (without them h is x).  y may be NULL when y8 is given; rstd (f32 [rows], = R) may be NULL when no backward follows.
  * y8 / scale8 (optional): the e4m3 copy of the UNROUNDED y in blocks of 128 features, as merlot_quantize_blocks lays it out (ld8 = ceil(H / 128) * 128). */
 int merlot_rms_fwd(const void* x, int64_t ldx, int x_f32, const void* residual, int64_t ldr, const float* gamma, void* h, void* y, float* rstd,

@@ -9,7 +9,7 @@
 // Measured (101376 x 768 bf16): forward with residual 117 us = 5.3 TB/s (a large copy: 4.85 TB/s), with the 8-bit copy in place of y 103 us, backward with
 // the residual stream's gradient 122 us with dgamma = 5.1 TB/s.  Widths that are whole slabs take code without per-element branches (FULL: backward 184 -> 120 us).
 // All sums are fp32.  The statistics are taken from h AS STORED (rounded to its type), so that the backward, which reads the stored h, differentiates the
-// function the forward computed.
+// function the forward computed.  A finite row has its norm whatever its magnitude: where the squares leave fp32's range the row is scaled first (rms_scaled).
 #include "common.h"
 #include "blocks8.h"
 
@@ -110,6 +110,49 @@ __device__ __forceinline__ float row_sum(float s, float (*red)[RowShape<LPR>::WP
     return s;
 }
 
+// largest value of the row's lanes (bit patterns of non-negative floats), the same in each of them; slot: as row_sum
+template <int LPR>
+__device__ __forceinline__ uint32_t row_umax(uint32_t m, float (*red)[RowShape<LPR>::WPR], int& slot) {
+    constexpr int WPR = RowShape<LPR>::WPR;
+#pragma unroll
+    for (int o = (LPR < 64 ? LPR : 64) / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+    if constexpr (WPR > 1) {
+        if ((threadIdx.x & 63) == 0) red[slot][threadIdx.x >> 6] = __uint_as_float(m);
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < WPR; ++w) m = max(m, __float_as_uint(red[slot][w]));
+        slot ^= 1;
+    }
+    return m;
+}
+
+// A finite row whose sum of squares leaves fp32 (over 3.4e38, or, with an eps to match, so small that squares lose bits): its values are scaled by a power of two that
+// brings the larger of max |v| and sqrt(eps) near 1, and the sum is taken again.  -> 1 / rms of the SCALED row; scale times that is 1 / rms.  Uniform over a row's lanes.
+template <int VEC, int NS, int LPR>
+__device__ __forceinline__ float rms_scaled(float (&v)[NS][VEC], float& scale, int H, float eps, float (*red)[RowShape<LPR>::WPR], int& slot) {
+    uint32_t m = 0u;
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) m = max(m, __float_as_uint(v[i][e]) & 0x7fffffffu);
+    m = row_umax<LPR>(m, red, slot);
+    scale = 1.f;
+    if (m <= 0x7f7fffffu) {                              // (with an infinity or NaN in the row the sum stays what it is)
+        const int e = min(max((int)(max(m, __float_as_uint(sqrtf(fabsf(eps)))) >> 23), 1), 253);
+        scale = __uint_as_float((uint32_t)(254 - e) << 23);
+    }
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < NS; ++i)
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            v[i][e] *= scale;
+            ss += v[i][e] * v[i][e];
+        }
+    ss = row_sum<LPR>(ss, red, slot);
+    return 1.0f / sqrtf(ss / (float)H + eps * scale * scale);
+}
+
 struct RmsFwdArgs {
     const void* x; int64_t ldx;
     const void* res; int64_t ldr;
@@ -154,8 +197,10 @@ __global__ __launch_bounds__(256) void rms_fwd_kernel(const RmsFwdArgs p) {
             for (int e = 0; e < VEC; ++e) ss += v[i][e] * v[i][e];
         }
         ss = row_sum<LPR>(ss, red, slot);
-        const float rstd = 1.0f / sqrtf(ss / (float)H + p.eps);
-        if (p.rstd && c0 == 0) p.rstd[row] = rstd;
+        const float ms = ss / (float)H + p.eps;
+        float rstd = 1.0f / sqrtf(ms), scale = 1.f;
+        if (!(ms >= 0x1p-90f && ms <= 3.402823466e38f)) rstd = rms_scaled<VEC, NS, LPR>(v, scale, H, p.eps, red, slot);
+        if (p.rstd && c0 == 0) p.rstd[row] = rstd * scale;
 #pragma unroll
         for (int i = 0; i < NS; ++i) {
             const int c = i * SLAB + c0;

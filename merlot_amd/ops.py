@@ -961,8 +961,8 @@ def _dense_like(x):
 
 
 def rms_norm_fwd(x, gamma, *, residual=None, out=True, q8=False, save_rstd=True, eps=1e-6):
-    """h = x + residual (rounded to x's type), R = 1 / sqrt(mean(h^2) + eps), y = h * R * gamma over the last dimension (1 ... 16 384 features).
-    x [..., H] bf16 or f32, residual like x (or None: h is x), gamma f32 [H].  -> (y, h, rstd, y8, scale8): y like x (None: out False); h None without a
+    """h = x + residual (rounded to x's type), R = 1 / sqrt(mean(h^2) + eps), y = h * R * gamma over the last dimension (1 ... 16 384 features),
+    for finite rows of any magnitude.  x [..., H] bf16 or f32, residual like x (or None: h is x), gamma f32 [H].  -> (y, h, rstd, y8, scale8): y like x (None: out False); h None without a
     residual; rstd f32 [rows] (None: save_rstd False); q8: y8 / scale8 = the e4m3 copy of the unrounded y in blocks of 128 features, as quantize_blocks
     lays it out -- the left operand of gemm_f8_blocks."""
     dt = x.dtype
