@@ -1175,9 +1175,10 @@ def clip_by_global_norm(grads, clip_norm, out=None):
     """every tensor times clip_norm / max(norm, clip_norm), norm = global_norm(grads); in place, or into `out` (tensors of the same shapes, f32 or bf16 each, that
     share no memory with each other or with other inputs).  grads, out: lists, or TensorLists a program keeps.  -> the norm BEFORE clipping (f32 scalar on the
     device).  An infinite norm scales by 0, a NaN one makes every element NaN."""
+    import ctypes
     clip_norm = float(clip_norm)
-    if not 0.0 < clip_norm < float('inf'):
-        raise ValueError(f"clip_norm: expected a positive finite number, got {clip_norm}")
+    if not 0.0 < ctypes.c_float(clip_norm).value < float('inf'):      # as the kernel gets it: under 2^-150 it would be 0, the norm alone
+        raise ValueError(f"clip_norm: expected a positive finite number in fp32's range, got {clip_norm}")
     grads = _tensor_list(grads)
     out = grads if out is None else _tensor_list(out)
     if out.shapes != grads.shapes:
