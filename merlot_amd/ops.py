@@ -1112,7 +1112,7 @@ def gemm_f8_blocks(a8, a_scale, b8, b_scale, *, bias=None, out=None, out_dtype=B
 
 class TensorList(object):
     """Many dense f32 / bf16 tensors of one device as ONE operand (global_norm, clip_by_global_norm): checked once, for as long as the tensors stay where they are.
-    Keeps their memory alive; a tensor whose storage has been exchanged since (`t.data = ...`) makes the next use raise."""
+    Keeps their memory alive; a tensor that has been given another storage, size or layout since (`t.data = ...`, `t.resize_(...)`) makes the next use raise."""
 
     def __init__(self, tensors):
         import ctypes
@@ -1133,15 +1133,17 @@ class TensorList(object):
         self.shapes = [t.shape for t in self.tensors]
         self.addresses = [t.data_ptr() for t in self.tensors]
         self.ptrs = (ctypes.c_int64 * n)(*self.addresses)
-        self.numels = (ctypes.c_int64 * n)(*[t.numel() for t in self.tensors])
+        self.counts = [t.numel() for t in self.tensors]
+        self.numels = (ctypes.c_int64 * n)(*self.counts)
         self.bf16 = bytes(1 if t.dtype == BF16 else 0 for t in self.tensors)
 
     def __len__(self):
         return len(self.tensors)
 
     def check(self):
-        if list(map(torch.Tensor.data_ptr, self.tensors)) != self.addresses:
-            raise ValueError("TensorList: a tensor's storage has changed since the list was made")
+        T, ts = torch.Tensor, self.tensors
+        if list(map(T.data_ptr, ts)) != self.addresses or list(map(T.numel, ts)) != self.counts or not all(map(T.is_contiguous, ts)):
+            raise ValueError("TensorList: a tensor's storage, size or layout has changed since the list was made")
 
 
 def _tensor_list(ts):
