@@ -960,6 +960,10 @@ def _dense_like(x):
     return torch.empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)     # (the first takes 1.2 us, the second 1.7)
 
 
+# (an iterable of tensors) a kernel has written them: autograd refuses a graph that saved one before, as after torch's own writes
+_written = torch._C._increment_version
+
+
 def rms_norm_fwd(x, gamma, *, residual=None, out=True, q8=False, save_rstd=True, eps=1e-6):
     """h = x + residual (rounded to x's type), R = 1 / sqrt(mean(h^2) + eps), y = h * R * gamma over the last dimension (1 ... 16 384 features),
     for finite rows of any magnitude.  x [..., H] bf16 or f32, residual like x (or None: h is x), gamma f32 [H].  -> (y, h, rstd, y8, scale8): y like x (None: out False); h None without a
@@ -1017,6 +1021,7 @@ def rms_norm_bwd(dy, h, rstd, gamma, dgamma, *, dres=None):
         ws = gamma.new_empty(nbytes // 4)
         call('merlot_rms_bwd', dy.data_ptr(), lddy, 1 if dt is F32 else 0, h.data_ptr(), ldh, rstd.data_ptr(), gamma.data_ptr(), _p(dres), lddr, dx.data_ptr(),
              dgamma.data_ptr(), rows, H, ws.data_ptr(), nbytes, _stream(dev))
+        _written((dgamma,))
     return dx
 
 
@@ -1082,7 +1087,8 @@ def gemm_f8_blocks(a8, a_scale, b8, b_scale, *, bias=None, out=None, out_dtype=B
     ldsa, ldsb = _scale_rows(a_scale, M, K // 128, dev, 'a_scale'), _scale_rows(b_scale, N, K // 128, dev, 'b_scale')
     if bias is not None:
         _dense(bias, N, dev, 'bias')
-    if out is None:
+    fresh = out is None
+    if fresh:
         if accumulate:
             raise ValueError("gemm_f8_blocks: accumulate needs out")
         if out_dtype is not BF16 and out_dtype is not F32:
@@ -1107,6 +1113,8 @@ def gemm_f8_blocks(a8, a_scale, b8, b_scale, *, bias=None, out=None, out_dtype=B
         TIMER.time('gemm_f8_blocks', 2.0 * M * N * K, lambda: call('merlot_gemm_f8_blocks', *args))
     else:
         call('merlot_gemm_f8_blocks', *args)
+    if not fresh:
+        _written((out,))
     return out
 
 
@@ -1187,4 +1195,6 @@ def clip_by_global_norm(grads, clip_norm, out=None):
         raise ValueError("clip_by_global_norm: out must hold tensors of the same shapes as grads")
     if out.device != grads.device:
         raise ValueError(f"clip_by_global_norm: out is on {out.device}, grads on {grads.device}")
-    return _clip(grads, clip_norm, out)
+    norm = _clip(grads, clip_norm, out)
+    _written(out.tensors)
+    return norm
