@@ -598,11 +598,11 @@ class LinearF8BlocksFn(torch.autograd.Function):
     backward are the one-byte transposed copies, not x."""
 
     @staticmethod
-    def forward(ctx, x, lin, grad_fmt):
+    def forward(ctx, x, lin, grad_fmt, graph):
         if lin.gb is not None and lin.w.shape[0] % 4 != 0:
             raise ValueError("linear_f8_blocks: a Linear with a bias needs an output width that is a multiple of 4 (the bias gradient's column sums)")
         x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
-        if ctx.needs_input_grad[0]:
+        if graph:
             w8, sw, wt8, swt = ops.quantize_blocks(lin.wb, tile=128, transpose=True)
             x8, sx, xt8, sxt = ops.quantize_blocks(x2, transpose=True)
         else:                                            # no graph: nothing waits for a backward
@@ -617,19 +617,20 @@ class LinearF8BlocksFn(torch.autograd.Function):
         xt8, sxt, wt8, swt = ctx.saved_tensors
         dy2 = dy.contiguous().view(-1, dy.shape[-1])
         if dy2.shape[0] == 0:
-            return torch.zeros(ctx.shape, device=dy.device, dtype=ctx.dtype), None, None
+            return torch.zeros(ctx.shape, device=dy.device, dtype=ctx.dtype), None, None, None
         d8, sd, dt8, sdt = ops.quantize_blocks(dy2, ctx.grad_fmt, transpose=True)
         ops.gemm_f8_blocks(dt8, sdt, xt8, sxt, out=lin.gw, accumulate=True)
         if lin.gb is not None:
             ops.colsum_bf16(dy2, lin.gb)
-        return ops.gemm_f8_blocks(d8, sd, wt8, swt, out_dtype=ctx.dtype).view(ctx.shape), None, None
+        return ops.gemm_f8_blocks(d8, sd, wt8, swt, out_dtype=ctx.dtype).view(ctx.shape), None, None, None
 
 
 def linear_f8_blocks(x, lin, grad_fmt=ops.F8_E4M3):
     """x [..., in] (bf16 or f32) -> bf16 [..., out]; weight and bias gradients are ACCUMULATED into the Linear's gradient views.  Operands are e4m3 with a scale per
     128 values along each product's reduction (activations) or per 128 x 128 tile (weights); grad_fmt: the format of dy.  As with every layer here whose parameters live
     in a store, the backward runs where x requires a gradient."""
-    return LinearF8BlocksFn.apply(x, lin, grad_fmt)
+    # (whether a backward may follow is known here only: inside an autograd function grad mode is off, and needs_input_grad does not look at it)
+    return LinearF8BlocksFn.apply(x, lin, grad_fmt, torch.is_grad_enabled() and x.requires_grad)
 
 
 class GatherAddFn(torch.autograd.Function):

@@ -1,0 +1,36 @@
+"""CPU: what layers.linear_f8_blocks asks of the 8-bit operators, with those operators replaced by ones that take notes."""
+import pytest
+import torch
+
+from merlot_amd import layers, ops
+
+
+class _Lin(object):
+    def __init__(self, n, k, bias):
+        self.w = torch.zeros(n, k)
+        self.wb, self.gw = self.w.bfloat16(), torch.zeros(n, k)
+        self.b = self.gb = torch.zeros(n) if bias else None
+
+
+@pytest.fixture
+def notes(monkeypatch):
+    made = []
+
+    def quantize(x, fmt=0, *, tile=1, rows=True, transpose=False):
+        made.append(transpose)
+        q, s = x.new_empty(x.shape), x.new_empty(1)
+        return (q, s, q.t().clone(), s.clone()) if transpose else (q, s)
+    monkeypatch.setattr(ops, 'quantize_blocks', quantize)
+    monkeypatch.setattr(ops, 'gemm_f8_blocks', lambda a, sa, b, sb, **kw: torch.zeros(a.shape[0], b.shape[0], dtype=torch.bfloat16))
+    return made
+
+
+def test_transposed_copies_only_where_a_backward_may_follow(notes):
+    lin = _Lin(8, 16, False)
+    x = torch.zeros(4, 16, requires_grad=True)
+    y = layers.linear_f8_blocks(x, lin)
+    assert y.requires_grad and notes == [True, True]
+    for call in (lambda: layers.linear_f8_blocks(x.detach(), lin), lambda: torch.no_grad()(layers.linear_f8_blocks)(x, lin)):
+        del notes[:]
+        y = call()
+        assert not y.requires_grad and y.shape == (4, 8) and notes == [False, False]
