@@ -599,8 +599,8 @@ class LinearF8BlocksFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, lin, grad_fmt, graph):
-        if lin.gb is not None and lin.w.shape[0] % 4 != 0:
-            raise ValueError("linear_f8_blocks: a Linear with a bias needs an output width that is a multiple of 4 (the bias gradient's column sums)")
+        if graph and lin.gb is not None and lin.w.shape[0] % 4 != 0:
+            raise ValueError("linear_f8_blocks: the backward of a Linear with a bias needs an output width that is a multiple of 4 (the bias gradient's column sums)")
         x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
         if graph:
             w8, sw, wt8, swt = ops.quantize_blocks(lin.wb, tile=128, transpose=True)

@@ -34,3 +34,14 @@ def test_transposed_copies_only_where_a_backward_may_follow(notes):
         del notes[:]
         y = call()
         assert not y.requires_grad and y.shape == (4, 8) and notes == [False, False]
+
+
+def test_any_output_width_without_a_backward(notes):
+    lin = _Lin(6, 16, True)
+    x = torch.zeros(4, 16, requires_grad=True)
+    with pytest.raises(ValueError, match='multiple of 4'):     # the bias gradient's column sums
+        layers.linear_f8_blocks(x, lin)
+    assert notes == []
+    with torch.no_grad():
+        assert layers.linear_f8_blocks(x, lin).shape == (4, 6)
+    assert layers.linear_f8_blocks(x.detach(), lin).shape == (4, 6)
