@@ -602,6 +602,9 @@ class LinearF8BlocksFn(torch.autograd.Function):
         if graph and lin.gb is not None and lin.w.shape[0] % 4 != 0:
             raise ValueError("linear_f8_blocks: the backward of a Linear with a bias needs an output width that is a multiple of 4 (the bias gradient's column sums)")
         x2 = x if x.dim() == 2 else x.reshape(-1, x.shape[-1])
+        if graph and max(x2.shape[0], lin.w.shape[0]) > ops.F8_BLOCKS_MAX_K:
+            raise ValueError(f"linear_f8_blocks: the backward's products run along the rows and the outputs, up to {ops.F8_BLOCKS_MAX_K} of them; "
+                             f"got {x2.shape[0]} rows and {lin.w.shape[0]} outputs")
         if graph:
             w8, sw, wt8, swt = ops.quantize_blocks(lin.wb, tile=128, transpose=True)
             x8, sx, xt8, sxt = ops.quantize_blocks(x2, transpose=True)

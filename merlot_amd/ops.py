@@ -1052,6 +1052,9 @@ def quantize_blocks(x, fmt=F8_E4M3, *, tile=1, rows=True, transpose=False):
     return (q, s, qt, st) if transpose else (q, s)
 
 
+F8_BLOCKS_MAX_K = (1 << 22) - 128                          # longest reduction of gemm_f8_blocks: operand rows lie under 2^22 bytes apart
+
+
 def _scale_rows(s, rows, nb, dev, name):
     """row stride of `rows` rows of nb scale bytes, read in whole words of 4"""
     if s.dtype is not torch.uint8 or s.get_device() != dev or s.shape != (rows, nb):

@@ -45,3 +45,19 @@ def test_any_output_width_without_a_backward(notes):
     with torch.no_grad():
         assert layers.linear_f8_blocks(x, lin).shape == (4, 6)
     assert layers.linear_f8_blocks(x.detach(), lin).shape == (4, 6)
+
+
+@pytest.mark.parametrize('rows', [(1 << 22) - 127, 1 << 22])
+def test_more_rows_than_the_weight_gradient_takes_are_refused_in_the_forward(notes, rows):
+    """(the product of the backward, whose reduction they are, refuses them: too late, the step's other gradients are on their way)"""
+    lin = _Lin(8, 1, False)
+    x = torch.zeros(rows, 1, dtype=torch.bfloat16, requires_grad=True)
+    with pytest.raises(ValueError, match='4194176'):
+        layers.linear_f8_blocks(x, lin)
+    assert notes == []
+    assert layers.linear_f8_blocks(x.detach(), lin).shape == (rows, 8)
+    assert layers.linear_f8_blocks(x[:ops.F8_BLOCKS_MAX_K], lin).requires_grad
+    d = ops.LIB.load()
+    P, K = 4096, ops.F8_BLOCKS_MAX_K                           # the product's own limit (refused before any launch)
+    call = lambda k, ws: (d.merlot_gemm_f8_blocks(P, k, 0, P, 1 << 15, P, k, P, 1 << 15, P, 8, 8, 8, k, 1, 0, None, None, ws, None), d.merlot_last_error().decode())  # noqa: E731
+    assert 'leading dimension' in call(K + 128, 0)[1] and 'workspace' in call(K, 0)[1]
