@@ -396,14 +396,13 @@ template <int ITER, bool RES, bool HOLD = false>
 __global__ __launch_bounds__(256, 2) void gn_fwd_fused_kernel(const bf16* __restrict__ x, const float* __restrict__ gamma,
                                                            const float* __restrict__ beta, const bf16* __restrict__ res,
                                                            bf16* __restrict__ y, float* __restrict__ stats, unsigned* __restrict__ ws,
-                                                           int N, int HW, int C, int G, int relu, int split, float inv_cnt, float eps, int static_items) {
+                                                           int N, int HW, int C, int G, int relu, int split, float inv_cnt, float eps) {
     extern __shared__ float gsm[];                         // [G][2] this slice's sums, then [G][2] {mean, rstd} of the sample
     __shared__ int s_item;
     unsigned* arrive = ws + 16;
     float* sums = reinterpret_cast<float*>(ws + 16 + gn_ws_arrive_words(N));
     const int tid = threadIdx.x, bd = blockDim.x;
-    // (static_items: experiments only -- item = workgroup id instead of a claim, scripts/exp_gn_slices.py: the test of the dispatch model in the GN_FUSED_MAX_SLICES comment)
-    if (tid == 0) s_item = static_items ? (int)blockIdx.x : (int)__hip_atomic_fetch_add(ws, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (tid == 0) s_item = (int)__hip_atomic_fetch_add(ws, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     for (int i = tid; i < 2 * G; i += bd) gsm[i] = 0.f;
     __syncthreads();
     const int item = s_item, n = item / split, sl = item - n * split;
@@ -516,14 +515,13 @@ __global__ __launch_bounds__(256, 2) void gn_bwd_fused_kernel(const bf16* __rest
                                                            const float* __restrict__ stats, const float* __restrict__ gamma,
                                                            const float* __restrict__ beta, float* __restrict__ dgamma, float* __restrict__ dbeta,
                                                            float* __restrict__ gsum, bf16* __restrict__ dx, bf16* __restrict__ dres,
-                                                           unsigned* __restrict__ ws, int N, int HW, int C, int G, int relu, int split, int static_items) {
+                                                           unsigned* __restrict__ ws, int N, int HW, int C, int G, int relu, int split) {
     extern __shared__ float gsm[];                         // [C][2] per-channel partials of this slice, then [G][2] the sample's gsum
     __shared__ int s_item, s_last;
     unsigned* arrive = ws + 16;
     float* slots = reinterpret_cast<float*>(ws + 16 + gn_ws_arrive_words(N));     // [N][split][C + G][2]
     const int tid = threadIdx.x, bd = blockDim.x;
-    // (static_items: experiments only -- item = workgroup id instead of a claim, scripts/exp_gn_slices.py: the test of the dispatch model in the GN_FUSED_MAX_SLICES comment)
-    if (tid == 0) s_item = static_items ? (int)blockIdx.x : (int)__hip_atomic_fetch_add(ws, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (tid == 0) s_item = (int)__hip_atomic_fetch_add(ws, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     for (int i = tid; i < 2 * (C + G); i += bd) gsm[i] = 0.f;
     __syncthreads();
     const int item = s_item, n = item / split, sl = item - n * split;
@@ -900,23 +898,11 @@ extern "C" int64_t merlot_groupnorm_fused_workspace_bytes(int N, int C, int G) {
 // slots fills it with waiters, the next workgroup in line is (within 8 ids) one for that XCD, and nothing starts any more -- the other XCDs drain and idle.  (Stalls that
 // resolve do so after ~20 s: something outside the kernel re-dispatches the waves.)  With S slices <= the per-XCD capacity C the same argument gives termination: a blocked
 // dispatcher means a full XCD; if the oldest unfinished sample still had unclaimed slices every resident workgroup would hold one of ITS slices, so C <= claimed < S.
-// The model predicts that with item = workgroup id (no claims) the round-robin itself spreads a sample over the eight XCDs and the limit becomes 8 C: measured with
-// MERLOT_GN_STATIC=1 in the experiments build (profiles/r06_z13_gn_static.txt) -- the 64-per-XCD backward runs at 70 / 132 / 256 / 480 slices and hangs at 520 and 640.
+// The model predicts that with item = workgroup id (no claims) the round-robin itself spreads a sample over the eight XCDs and the limit becomes 8 C: a form of the kernels
+// that is not kept bore that out (profiles/r06_z13_gn_static.txt) -- the 64-per-XCD backward ran at 70 / 132 / 256 / 480 slices and hung at 520 and 640.
 // Hence: both kernels are compiled for >= 2 workgroups per CU (__launch_bounds__(256, 2): C >= 64; tests/test_loop_isa.py checks the register counts) and both entries
 // refuse more than 40 slices.  Every as-shipped forward shape is <= 33; the forward default ran 3 900 individually timed calls without an outlier.
 constexpr int GN_FUSED_MAX_SLICES = 40;
-static int gn_static_items() {
-#ifdef MERLOT_EXPERIMENTS
-    if (const char* e = getenv("MERLOT_GN_STATIC")) return atoi(e);
-#endif
-    return 0;
-}
-static int gn_fused_max_slices() {
-#ifdef MERLOT_EXPERIMENTS
-    if (const char* e = getenv("MERLOT_GN_MAX_SLICES")) return atoi(e);       // scripts/exp_gn_slices.py: where the stall begins
-#endif
-    return GN_FUSED_MAX_SLICES;
-}
 // the backward's workspace: control words + one slot of (C + G) float pairs per (sample, slice); the slicing is the launch's own (GN_BWD_ITER positions per thread)
 constexpr int GN_BWD_ITER = 8;
 extern "C" int64_t merlot_groupnorm_bwd_fused_workspace_bytes(int N, int H, int W, int C, int G) {
@@ -940,11 +926,11 @@ extern "C" int merlot_groupnorm_fwd_fused(const void* x, const float* gamma, con
     const int HW = H * W;
     const int threads = gn_block_threads(C);
     const int pstep = threads / (C / 8);
-    const bool hold = res && (HW + 8 * pstep - 1) / (8 * pstep) <= gn_fused_max_slices();      // (see the kernel: the residual held across the wait, or read behind it)
+    const bool hold = res && (HW + 8 * pstep - 1) / (8 * pstep) <= GN_FUSED_MAX_SLICES;      // (see the kernel: the residual held across the wait, or read behind it)
     const int iter = hold ? 8 : 16;
     const int split = (HW + iter * pstep - 1) / (iter * pstep);
     MERLOT_CHECK((int64_t)N * split < (1LL << 31), MERLOT_ESHAPE, "merlot_groupnorm_fwd_fused: too many slices");
-    MERLOT_CHECK(split <= gn_fused_max_slices(), MERLOT_ESHAPE, "merlot_groupnorm_fwd_fused: %d slices per sample (H * W = %d positions of %d channels); measured up to %d -- use merlot_groupnorm_fwd",
+    MERLOT_CHECK(split <= GN_FUSED_MAX_SLICES, MERLOT_ESHAPE, "merlot_groupnorm_fwd_fused: %d slices per sample (H * W = %d positions of %d channels); measured up to %d -- use merlot_groupnorm_fwd",
                  split, HW, C, GN_FUSED_MAX_SLICES);
     hipError_t e = hipMemsetAsync(ws, 0, 4 * (16 + gn_ws_arrive_words(N) + (size_t)N * 2 * G), (hipStream_t)stream);
     MERLOT_CHECK(e == hipSuccess, MERLOT_ELAUNCH, "hipMemsetAsync: %s", hipGetErrorString(e));
@@ -952,13 +938,13 @@ extern "C" int merlot_groupnorm_fwd_fused(const void* x, const float* gamma, con
     const size_t lds = sizeof(float) * 4 * G;
     if (res && hold)
         hipLaunchKernelGGL((gn_fwd_fused_kernel<8, true, true>), dim3(N * split), dim3(threads), lds, (hipStream_t)stream, (const bf16*)x, gamma, beta,
-                           (const bf16*)res, (bf16*)y, stats, (unsigned*)ws, N, HW, C, G, relu, split, inv_cnt, eps, gn_static_items());
+                           (const bf16*)res, (bf16*)y, stats, (unsigned*)ws, N, HW, C, G, relu, split, inv_cnt, eps);
     else if (res)
         hipLaunchKernelGGL((gn_fwd_fused_kernel<16, true>), dim3(N * split), dim3(threads), lds, (hipStream_t)stream, (const bf16*)x, gamma, beta,
-                           (const bf16*)res, (bf16*)y, stats, (unsigned*)ws, N, HW, C, G, relu, split, inv_cnt, eps, gn_static_items());
+                           (const bf16*)res, (bf16*)y, stats, (unsigned*)ws, N, HW, C, G, relu, split, inv_cnt, eps);
     else
         hipLaunchKernelGGL((gn_fwd_fused_kernel<16, false>), dim3(N * split), dim3(threads), lds, (hipStream_t)stream, (const bf16*)x, gamma, beta,
-                           (const bf16*)nullptr, (bf16*)y, stats, (unsigned*)ws, N, HW, C, G, relu, split, inv_cnt, eps, gn_static_items());
+                           (const bf16*)nullptr, (bf16*)y, stats, (unsigned*)ws, N, HW, C, G, relu, split, inv_cnt, eps);
     return merlot_launch_status("merlot_groupnorm_fwd_fused");
 }
 
@@ -979,8 +965,8 @@ extern "C" int merlot_groupnorm_bwd_fused(const void* dy, const void* y, const v
     constexpr int ITER = GN_BWD_ITER;
     const int split = (HW + ITER * pstep - 1) / (ITER * pstep);
     MERLOT_CHECK((int64_t)N * split < (1LL << 31), MERLOT_ESHAPE, "merlot_groupnorm_bwd_fused: too many slices");
-    // 66 slices per sample: calls that never return (profiles/r06_z6_gn_stress.txt; cause not found -- every shape up to 33 slices ran, thousands of calls forward)
-    MERLOT_CHECK(split <= gn_fused_max_slices(), MERLOT_ESHAPE, "merlot_groupnorm_bwd_fused: %d slices per sample (H * W = %d positions of %d channels); this entry stalls above %d -- use merlot_groupnorm_bwd",
+    // 66 slices per sample: calls that never return (profiles/r06_z6_gn_stress.txt; the cause: GN_FUSED_MAX_SLICES)
+    MERLOT_CHECK(split <= GN_FUSED_MAX_SLICES, MERLOT_ESHAPE, "merlot_groupnorm_bwd_fused: %d slices per sample (H * W = %d positions of %d channels); this entry stalls above %d -- use merlot_groupnorm_bwd",
                  split, HW, C, GN_FUSED_MAX_SLICES);
     hipError_t e = hipMemsetAsync(ws, 0, 4 * (16 + gn_ws_arrive_words(N)), (hipStream_t)stream);      // the control words; every slot and gsum entry is written before it is read
     MERLOT_CHECK(e == hipSuccess, MERLOT_ELAUNCH, "hipMemsetAsync: %s", hipGetErrorString(e));
@@ -988,11 +974,11 @@ extern "C" int merlot_groupnorm_bwd_fused(const void* dy, const void* y, const v
     const bool has_y = relu && y != nullptr;
     if (has_y)
         hipLaunchKernelGGL((gn_bwd_fused_kernel<ITER, true>), dim3(N * split), dim3(threads), lds, (hipStream_t)stream, (const bf16*)dy, (const bf16*)y,
-                           (const bf16*)x, stats, gamma, beta, dgamma, dbeta, gsum, (bf16*)dx, (bf16*)dres, (unsigned*)ws, N, HW, C, G, relu, split, gn_static_items());
+                           (const bf16*)x, stats, gamma, beta, dgamma, dbeta, gsum, (bf16*)dx, (bf16*)dres, (unsigned*)ws, N, HW, C, G, relu, split);
     else
         hipLaunchKernelGGL((gn_bwd_fused_kernel<ITER, false>), dim3(N * split), dim3(threads), lds, (hipStream_t)stream, (const bf16*)dy,
                            (const bf16*)nullptr, (const bf16*)x, stats, gamma, beta, dgamma, dbeta, gsum, (bf16*)dx, (bf16*)dres, (unsigned*)ws, N,
-                           HW, C, G, relu, split, gn_static_items());
+                           HW, C, G, relu, split);
     return merlot_launch_status("merlot_groupnorm_bwd_fused");
 }
 
