@@ -11,10 +11,10 @@ FLAGS="--offload-arch=gfx950 -O3 -std=c++17 -fPIC -Xclang -target-feature -Xclan
 SRCS="gemm attention layernorm elementwise index conv conv_gemm image fp8 jpeg rmsnorm blocks8 gemm_blocks clip"
 HDRS="common.h blocks8.h gemm_ring.h gemm_p8.inc gemm_q8.inc attention_res.inc attention_fb.inc attention_pp.inc ../../include/merlot_hip.h"
 
-newer() {  # newer <target> <deps...>: true when target is missing or older than a dependency
+newer() {  # newer <target> <deps...>: true when target is missing or older than a dependency -- this file, which holds the flags, is one of all of them --, or MERLOT_BUILD_ALL=1
   local t=$1; shift
-  [ ! -f "$t" ] && return 0
-  for d in "$@"; do [ "$d" -nt "$t" ] && return 0; done
+  [ ! -f "$t" ] || [ "$MERLOT_BUILD_ALL" = 1 ] && return 0
+  for d in build.sh "$@"; do [ "$d" -nt "$t" ] && return 0; done
   return 1
 }
 
