@@ -585,7 +585,7 @@ int merlot_gemm_f8_blocks(const void* A8, int64_t lda, int fmt_a, const uint8_t*
 
 /* norm[0] (f32) = sqrt(sum over n tensors of sum of g^2), summed in 64 bits in a fixed order, and with clip > 0 out = g * (clip / max(norm, clip)) -- the
  * arithmetic of tf.clip_by_global_norm (utils/optimization.py:233-237); clip 0: the norm alone, `out` may be NULL.  in / out / numel / types: HOST arrays of n
- * device addresses, element counts (0 allowed) and types (bit 0: in is bf16, bit 1: out is bf16; otherwise f32); addresses aligned to their type.  out[i] == in[i]
+ * device addresses, element counts (0 allowed) and types (bit 0: in is bf16, bit 1: out is bf16; otherwise f32), under 2^43 elements in all, each tensor counted in whole 4 096s; addresses aligned to their type.  out[i] == in[i]
  * of the same type works in place; outputs that overlap each other or another tensor's input are refused.  A norm that is not finite is passed on: infinity
  * scales by 0, NaN by NaN.  workspace: merlot_clip_workspace_bytes(n) bytes, 8-byte aligned, any content. */
 int64_t merlot_clip_workspace_bytes(int64_t n);

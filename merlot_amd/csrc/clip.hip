@@ -169,6 +169,9 @@ __global__ __launch_bounds__(256) void clip_scale_table_kernel(const ClipEntry* 
     clip_scale_all(t, count, chunks, part, nparts, clip, norm);
 }
 
+// chunks of a tensor at that address (groups start at multiples of 16 bytes)
+uint64_t clip_chunks(int64_t address, int64_t numel, int size) { return ((uint64_t)numel + ((uint64_t)address & 15) / size + CLIP_CHUNK - 1) / CLIP_CHUNK; }
+
 struct Span { uint64_t lo, hi; };
 
 }  // namespace
@@ -184,12 +187,15 @@ extern "C" int merlot_clip_by_global_norm(const int64_t* in, const int64_t* out,
     MERLOT_CHECK(clip == 0.f || out, MERLOT_ESHAPE, "merlot_clip_by_global_norm: null operand");
     MERLOT_CHECK(workspace && workspace_bytes >= merlot_clip_workspace_bytes(n), MERLOT_ESHAPE, "merlot_clip_by_global_norm: workspace too small");
     MERLOT_CHECK(((uintptr_t)workspace & 7) == 0, MERLOT_EALIGN, "merlot_clip_by_global_norm: workspace must be 8-byte aligned");
+    uint64_t all = 0;
     for (int64_t i = 0; i < n; ++i) {
         MERLOT_CHECK(numel[i] >= 0 && numel[i] < ((int64_t)1 << 40), MERLOT_ESHAPE, "merlot_clip_by_global_norm: tensor %lld has a bad size", (long long)i);
         MERLOT_CHECK(types[i] < 4, MERLOT_EDTYPE, "merlot_clip_by_global_norm: tensor %lld has a bad type", (long long)i);
         MERLOT_CHECK(numel[i] == 0 || (in[i] && (clip == 0.f || out[i])), MERLOT_ESHAPE, "merlot_clip_by_global_norm: null tensor %lld", (long long)i);
         const int si = types[i] & 1 ? 2 : 4, so = types[i] & 2 ? 2 : 4;
         MERLOT_CHECK(in[i] % si == 0 && (clip == 0.f || out[i] % so == 0), MERLOT_EALIGN, "merlot_clip_by_global_norm: tensor %lld is not aligned to its type", (long long)i);
+        if (numel[i]) all += clip_chunks(in[i], numel[i], si);
+        MERLOT_CHECK(all < ((uint64_t)1 << 31) && i < (1 << 30), MERLOT_ESHAPE, "merlot_clip_by_global_norm: 2^43 elements or more (each tensor counted in whole 4096s), or 2^30 tensors, in one call");
     }
     if (clip > 0.f) {
         // an element written twice, or read after it was written, would be scaled twice or raced for: each output is an output once, and shares bytes with
@@ -229,12 +235,9 @@ extern "C" int merlot_clip_by_global_norm(const int64_t* in, const int64_t* out,
     uint64_t chunks = 0;
     for (int64_t i = 0; i < n; ++i) {
         if (numel[i] == 0) continue;
-        const int es = types[i] & 1 ? 2 : 4;
-        const uint64_t elements = (uint64_t)numel[i] + ((uint64_t)in[i] & 15) / es;       // (groups start at multiples of 16 bytes)
         t.e[count - filled] = {(const void*)in[i], clip > 0.f ? (void*)out[i] : nullptr, numel[i], (uint32_t)chunks, types[i]};
         ++count;
-        chunks += (elements + CLIP_CHUNK - 1) / CLIP_CHUNK;
-        MERLOT_CHECK(chunks < ((uint64_t)1 << 31) && count < (1 << 30), MERLOT_ESHAPE, "merlot_clip_by_global_norm: 64 TiB in one call");
+        chunks += clip_chunks(in[i], numel[i], types[i] & 1 ? 2 : 4);
         if (table && count - filled == CLIP_TENSORS) {
             hipLaunchKernelGGL(clip_table_kernel, dim3(1), dim3(128), 0, s, t, table + filled, CLIP_TENSORS);
             filled = count;
