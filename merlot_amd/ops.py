@@ -921,7 +921,7 @@ def _rows(t, dtype, dev, name):
     if t.get_device() != dev:
         raise ValueError(f"{name}: expected a tensor on cuda:{dev}, the current device, got {t.device}")
     strides = t.stride()
-    if not strides or strides[-1] != 1:
+    if not strides or strides[-1] != 1 and t.shape[-1] != 1:
         raise ValueError(f"{name}: last dim must be contiguous")
     if len(strides) != 2:
         cols = t.shape[-1]
@@ -1060,7 +1060,7 @@ def _scale_rows(s, rows, nb, dev, name):
     if s.dtype is not torch.uint8 or s.get_device() != dev or s.shape != (rows, nb):
         raise ValueError(f"{name}: expected [{rows}, {nb}] scale bytes (uint8) on cuda:{dev}, got {tuple(s.shape)} {s.dtype} on {s.device}")
     ld, one = s.stride()
-    if one != 1:
+    if one != 1 and nb != 1:
         raise ValueError(f"{name}: last dim must be contiguous")
     whole = (nb + 3) // 4 * 4
     if rows <= 1:
