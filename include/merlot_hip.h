@@ -557,7 +557,8 @@ int64_t merlot_example_index(const void* buf, int64_t n, int64_t* rows, int64_t 
 int merlot_rms_fwd(const void* x, int64_t ldx, int x_f32, const void* residual, int64_t ldr, const float* gamma, void* h, void* y, float* rstd,
                    void* y8, int64_t ld8, uint8_t* scale8, int64_t ld_scale8, int64_t rows, int H, float eps, merlot_stream_t stream);
 /* dx = R * (dy * gamma - n * mean(dy * gamma * n)) (+ dres), n = h * R; dgamma[H] (f32) += sum over rows of dy * n, in a fixed order (no atomics).  dy, h, dres
- * (may be NULL) and dx share one type; dx dense.  dx is the gradient of x and of the residual alike.  workspace: merlot_rms_bwd_workspace_bytes(rows, H), any content. */
+ * (may be NULL) and dx share one type; dx dense.  dx is the gradient of x and of the residual alike.  Sums are fp32: of |dy * gamma * n| over
+ * a row, of |dy * n| over the rows.  workspace: merlot_rms_bwd_workspace_bytes(rows, H), any content. */
 int64_t merlot_rms_bwd_workspace_bytes(int64_t rows, int H);
 int merlot_rms_bwd(const void* dy, int64_t lddy, int is_f32, const void* h, int64_t ldh, const float* rstd, const float* gamma, const void* dres,
                    int64_t lddr, void* dx, float* dgamma, int64_t rows, int H, void* workspace, int64_t workspace_bytes, merlot_stream_t stream);

@@ -631,7 +631,7 @@ class LinearF8BlocksFn(torch.autograd.Function):
 def linear_f8_blocks(x, lin, grad_fmt=ops.F8_E4M3):
     """x [..., in] (bf16 or f32) -> bf16 [..., out]; weight and bias gradients are ACCUMULATED into the Linear's gradient views.  Operands are e4m3 with a scale per
     128 values along each product's reduction (activations) or per 128 x 128 tile (weights); grad_fmt: the format of dy.  As with every layer here whose parameters live
-    in a store, the backward runs where x requires a gradient."""
+    in a store, the backward runs where x requires a gradient; it takes up to ops.F8_BLOCKS_MAX_K rows and outputs and, with a bias, outputs that are a multiple of 4."""
     # (whether a backward may follow is known here only: inside an autograd function grad mode is off, and needs_input_grad does not look at it)
     return LinearF8BlocksFn.apply(x, lin, grad_fmt, torch.is_grad_enabled() and x.requires_grad)
 
